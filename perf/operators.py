@@ -191,10 +191,11 @@ def _token_parts(s):
     return valid, safe, x, e, total, torch.log(total)
 
 
-def _alternatives(x, logtotal, valid, n):
-    """the ``n`` largest of each row, ties to the lowest index: one whole number orders both"""
+def _alternatives(logits, x, logtotal, valid, n):
+    """the ``n`` largest of each row, ties to the lowest index: one whole number orders both (of
+    the logits themselves: their distances from the largest, rounded, may tie where they don't)"""
     V = x.shape[1]
-    bits = (x + 0.0).view(torch.int32).long()
+    bits = (logits.float() + 0.0).view(torch.int32).long()
     order = torch.where(bits < 0, -(bits & 0x7FFFFFFF), bits)
     key = (order << 32) - torch.arange(V, device=x.device)
     idx = (-torch.topk(key, n, dim=1)[0]) & 0xFFFFFFFF
@@ -212,7 +213,7 @@ def _score(s, parts=None):
     mean = (e * torch.where(e > 0, x, torch.zeros_like(x))).sum(1) / total[:, 0]
     entropy = torch.where(empty, zero, logtotal[:, 0] - mean)
     n = s["case"]["top"]
-    top_logp, top_ids = _alternatives(x, logtotal, valid, n) if n else (x.new_empty((x.shape[0], 0)), safe.new_empty((x.shape[0], 0)))
+    top_logp, top_ids = _alternatives(s["logits"], x, logtotal, valid, n) if n else (x.new_empty((x.shape[0], 0)), safe.new_empty((x.shape[0], 0)))
     return {"logp": torch.where(valid, logp, zero), "entropy": torch.where(valid, entropy, zero), "top_logp": top_logp, "top_ids": top_ids}
 
 
@@ -355,9 +356,9 @@ def _exact_tokens(case, s):
         where = torch.arange(len(on), device=dev)
         logp[a + on], ent[a + on] = lq[where, t], h
         if n:
-            val, idx = torch.sort(lq, dim=1, descending=True, stable=True)
-            tv[a + on], ti[a + on] = val[:, :n], idx[:, :n]
-            del val, idx
+            idx = torch.sort(z, dim=1, descending=True, stable=True)[1][:, :n]
+            tv[a + on], ti[a + on] = lq.gather(1, idx), idx
+            del idx
         if train:
             g = s["grad"][a:b][on].double()
             d = -q * (g[:, :1] + g[:, 2:].sum(1, keepdim=True)) - g[:, 1:2] * (plogp + q * h[:, None])
