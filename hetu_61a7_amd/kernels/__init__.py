@@ -87,6 +87,13 @@ def check(ret, name=''):
         raise RuntimeError('HIP kernel %s failed with hipError %d' % (name, ret))
 
 
+def check_device(t, name=''):
+    """a launch goes to the current device: tensors of another one are refused, not read from it"""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError('%s: tensors on %s, but the current device is cuda:%d'
+                         % (name, t.device, torch.cuda.current_device()))
+
+
 def supported_float(t) -> bool:
     return t.dtype in (torch.float32, torch.bfloat16)
 

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import torch
 
-from . import fn, native, stream_ptr, check, P, I64, I32, F32
+from . import fn, native, stream_ptr, check, check_device, ptr, P, I64, I32, F32
 
 MODES = dict(sgd=0, momentum=1, nesterov=2, adagrad=3, adam=4, adamw=5, lamb=6)
 
@@ -33,7 +33,7 @@ def optimizer_flat(mode, p, g, s1=None, s2=None, shadow=None, lr=0.01, l2=0.0, m
                 dyn.data_ptr() if dyn is not None else None, stream_ptr()), 'optimizer')
         return
     if dyn is not None:
-        lr, beta1t, beta2t, gscale = [float(v) for v in dyn.tolist()]
+        lr, beta1t, beta2t, gscale = [float(v) for v in dyn.tolist()[:4]]
     from . import cpu_native
     if mode != 'lamb' and cpu_native.active(p, g) and p.is_contiguous() and g.is_contiguous():
         cpu_native.optimizer(mode, p, g, s1, s2, lr, l2, mu, beta1, beta2, beta1t, beta2t, eps, wd, gscale)
@@ -71,6 +71,133 @@ def optimizer_flat(mode, p, g, s1=None, s2=None, shadow=None, lr=0.01, l2=0.0, m
                 p[a:b].sub_(lr * ratio * (u[a:b] + wd * p[a:b]))
     if shadow is not None:
         shadow.copy_(p)
+
+
+# ---- AdamW with both moments in 8 bits (adamw8.hip) ---------------------------------------------
+STATE8_BLOCK = 256      # consecutive elements that share the moments' scales
+
+
+_M64 = (1 << 64) - 1
+
+
+def _i64(seed):
+    """the low 64 bits as a signed launch argument"""
+    seed = int(seed) & _M64
+    return seed - (1 << 64) if seed >> 63 else seed
+
+
+def step_seed(seed, step):
+    """the rounding seed of one step"""
+    return (int(seed) + int(step) * 0x9E3779B97F4A7C15) & _M64
+
+
+def adamw8_state(n, device):
+    """(m, v, m_scale, v_scale) of ``n`` weights before their first step: all zero.  ``m`` holds
+    float8_e4m3fn, ``v`` float8_e5m2 values; element i stands for value[i] * scale[i // 256]."""
+    from .. import native_array as _NA
+    nb = -(-int(n) // STATE8_BLOCK)
+    return (_NA.zeros(int(n), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+            _NA.zeros(int(n), dtype=torch.uint8, device=device).view(torch.float8_e5m2),
+            _NA.zeros(nb, dtype=torch.float32, device=device), _NA.zeros(nb, dtype=torch.float32, device=device))
+
+
+def state8_values(q, scale):
+    """the fp32 values that an 8-bit moment stands for"""
+    return q.float() * scale.repeat_interleave(STATE8_BLOCK)[:q.numel()]
+
+
+def state8_from_values(x, which):
+    """(8-bit values, block scales) nearest to fp32 ``x``: a moment's form ('s1': the first, 's2':
+    the second) made from 32 bits, as when a checkpoint with 32-bit moments is resumed"""
+    first = which == 's1'
+    x = x.reshape(-1).float()
+    nb = -(-x.numel() // STATE8_BLOCK)
+    scale = _scale8(x, nb, 7 if first else 14)
+    y = x / scale.repeat_interleave(STATE8_BLOCK)[:x.numel()]
+    if not first:       # the smallest value above 0 stays above 0
+        y = torch.where((x > 0) & (y < 2.0 ** -16), torch.full_like(y, 2.0 ** -16), y)
+    return y.to(torch.float8_e4m3fn if first else torch.float8_e5m2), scale
+
+
+def _round_bits(n, seed, device):
+    """adamw8.hip ``round_bits`` of elements 0 .. n - 1"""
+    h = (torch.arange(n, device=device) * 0x9E3779B1 + seed) & 0xFFFFFFFF
+    h = ((h ^ (h >> 16)) * 0x7FEB352D) & 0xFFFFFFFF
+    h = ((h ^ (h >> 15)) * 0x846CA68B) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+def _encode8(y, r16, mant, bias):
+    """adamw8.hip ``encode8``"""
+    cut = 23 - mant
+    r = ((r16 << (cut - 16)) | (1 << (cut - 17))).int()
+    y = torch.where(torch.isfinite(y), y, torch.zeros_like(y))
+    normal = ((y.view(torch.int32) + r) >> cut) - ((127 - bias) << mant)
+    small = ((y * 2.0 ** (bias + 22)).int() + r) >> cut
+    return torch.where(y < 2.0 ** (1 - bias), small, normal)
+
+
+def _scale8(x, nb, top):
+    x = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x))
+    x = torch.nn.functional.pad(x, (0, nb * STATE8_BLOCK - x.numel())).view(nb, STATE8_BLOCK)
+    return (((x.amax(1).view(torch.int32) >> 23) - top).clamp_min(1) << 23).view(torch.float32)
+
+
+def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.999, beta1t=0.0, beta2t=0.0,
+           eps=1e-7, wd=0.0, gscale=1.0, seed=0, dyn=None):
+    """One AdamW step of the flat fp32 weights ``p`` from the flat fp32 gradients ``g``, in place,
+    with both moments in 8 bits (``adamw8_state``).
+
+    The update takes the fresh moments in 32 bits; what is stored of them is rounded at random,
+    by bits that a hash of ``seed`` (64 bits) and the element's index gives: another seed every
+    step.  ``dyn``: fp32 {lr, beta1t, beta2t, gscale, step, 1 - beta1t, 1 - beta2t} on the device
+    instead of the arguments, for a captured step; the seed is then moved by ``step`` as
+    ``step_seed`` moves it.
+    ``shadow`` (bf16, the weights' copy) is written too.  A block of 256 shares one scale: where
+    several tensors share the buffer, start each at a multiple of 256."""
+    n = p.numel()
+    nb = -(-n // STATE8_BLOCK)
+    for t, dt, size, what in ((p, torch.float32, n, 'p'), (g, torch.float32, n, 'g'), (m, torch.float8_e4m3fn, n, 'm'),
+                              (v, torch.float8_e5m2, n, 'v'), (m_scale, torch.float32, nb, 'm_scale'),
+                              (v_scale, torch.float32, nb, 'v_scale'), (shadow, torch.bfloat16, n, 'shadow'),
+                              (dyn, torch.float32, 7, 'dyn')):
+        if t is None:
+            continue
+        if t.dtype != dt or t.numel() != size or not t.is_contiguous() or t.device != p.device:
+            raise ValueError('adamw8: %s has to be a contiguous %s of %d elements on %s, got %s %s on %s'
+                             % (what, dt, size, p.device, t.dtype, tuple(t.shape), t.device))
+    if n == 0:
+        return
+    if native(p):
+        check_device(p, 'adamw8')
+        f = fn('hetu_adamw8', [P, P, P, P, P, P, P, I64] + [F32] * 10 + [P, I64, P])
+        check(f(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale.data_ptr(), v_scale.data_ptr(),
+                ptr(shadow), n, lr, beta1, beta2, 1.0 - beta1, 1.0 - beta2, 1.0 - beta1t, 1.0 - beta2t, eps,
+                wd, gscale, ptr(dyn), _i64(seed), stream_ptr()), 'adamw8')
+        return
+    if dyn is not None:
+        lr, _, _, gscale, step, c1, c2 = [float(x) for x in dyn.tolist()]
+        seed = step_seed(seed, step)
+    else:
+        c1, c2 = 1.0 - beta1t, 1.0 - beta2t
+    key = int(seed) & _M64
+    r = _round_bits(n, (key ^ (key >> 32)) & 0xFFFFFFFF, p.device)
+    gr = g * gscale
+    m1 = beta1 * state8_values(m, m_scale) + (1 - beta1) * gr
+    v1 = beta2 * state8_values(v, v_scale) + (1 - beta2) * gr * gr
+    u = (m1 / c1) / (torch.sqrt(v1 / c2) + eps)
+    p.sub_(lr * (u + wd * p))
+    if shadow is not None:
+        shadow.copy_(p)
+    m_scale.copy_(_scale8(m1, nb, 7))
+    v_scale.copy_(_scale8(v1, nb, 14))
+    mc = _encode8(m1.abs() / m_scale.repeat_interleave(STATE8_BLOCK)[:n], r & 0xFFFF, 3, 7)
+    mc = torch.where(torch.isfinite(m1), mc, torch.full_like(mc, 0x7F)) | ((m1 < 0).int() << 7)
+    vc = _encode8(v1 / v_scale.repeat_interleave(STATE8_BLOCK)[:n], r >> 16, 2, 15)
+    vc = torch.where(v1 > 0, vc.clamp_min(1), vc)
+    vc = torch.where(torch.isnan(v1), torch.full_like(vc, 0x7F), torch.where(torch.isinf(v1), torch.full_like(vc, 0x7C), vc))
+    m.view(torch.uint8).copy_(mc)
+    v.view(torch.uint8).copy_(vc)
 
 
 SPARSE_MODES = dict(sgd=0, momentum=1, nesterov=2, adagrad=3, adam=4, adamw=5)

@@ -109,6 +109,12 @@ def next_seed(key, on_gpu=True):
     return s or 1
 
 
+def fixed_seed(key, place=0):
+    """a seed of op ``key`` that is the same in every step: for kernels that take the step number
+    from elsewhere"""
+    return _mix(_BASE[0] ^ _mix((int(key) << 20) ^ 0xF1) ^ _mix(int(place)))
+
+
 # ---- random fills / channel dropout ---------------------------------------------------------
 def uniform_(t, lo=0.0, hi=1.0, seed=None, key=0):
     """t ~ U[lo, hi) in place (fp32 / bf16 device tensor, contiguous)"""

@@ -82,6 +82,7 @@ class Optimizer(object):
     # flat update -------------------------------------------------------------------
     mode = 'sgd'
     n_states = 0
+    state_bits = 32     # 8: AdamWOptimizer(state_bits=8)
 
     def hyper(self, step):
         return dict(lr=self.get_learning_rate(), l2=self.l2reg)
@@ -90,6 +91,12 @@ class Optimizer(object):
         KO.optimizer_flat(self.mode, flat.param, flat.grad, flat.s1, flat.s2, flat.shadow,
                           gscale=flat.gscale, seg_off=flat.seg_off, seg_off_host=flat.seg_host,
                           norms_ws=flat.norms_ws, dyn=dyn, **self.hyper(step))
+
+    def shard_update(self, flat, lo, hi, own, step, dyn=None):
+        """ZeRO-1: update parameters [lo, hi) from ``flat.zgrad[own]`` with this rank's state"""
+        KO.optimizer_flat(self.mode, flat.param[lo:hi], flat.zgrad[own], flat.s1[own] if flat.s1 is not None else None,
+                          flat.s2[own] if flat.s2 is not None else None, None, gscale=flat.gscale, dyn=dyn,
+                          **self.hyper(step))
 
     def sparse_update(self, table, state, ids, grads, step):
         h = self.hyper(step)
@@ -158,9 +165,16 @@ class AdamOptimizer(Optimizer):
 
 
 class AdamWOptimizer(AdamOptimizer):
-    def __init__(self, learning_rate=0.01, beta1=0.9, beta2=0.999, epsilon=1e-7, weight_decay=0):
+    """AdamW.  ``state_bits=8`` keeps the moments of the dense parameters in 8 bits with one scale
+    for each 256 elements, stochastically rounded (``kernels.optim.adamw8``): 2 bytes a parameter
+    instead of 8, and 12 fewer to move a step.  Row-sparse (embedding) parameters keep fp32 moments."""
+
+    def __init__(self, learning_rate=0.01, beta1=0.9, beta2=0.999, epsilon=1e-7, weight_decay=0, state_bits=32):
         super().__init__(learning_rate, beta1, beta2, epsilon, 0)
+        if state_bits not in (8, 32):
+            raise ValueError('AdamWOptimizer: state_bits is 8 or 32, got %r' % (state_bits,))
         self.weight_decay = weight_decay
+        self.state_bits = state_bits
         self.name = 'AdamW'
         self.mode = 'adamw'
 
@@ -168,6 +182,30 @@ class AdamWOptimizer(AdamOptimizer):
         h = super().hyper(step)
         h['wd'] = self.weight_decay
         return h
+
+    def _update8(self, flat, param, grad, own, shadow, step, dyn):
+        """one adamw8 launch over flat elements ``own`` of the state.  The rounding's seed follows
+        from the run's seed, the place and the step number alone: the same on every replica, in a
+        replayed step, and after a resume."""
+        from .kernels import rng
+        seed = rng.fixed_seed(flat.rng_key, own.start)
+        if dyn is None:
+            seed = KO.step_seed(seed, step)
+        blocks = slice(own.start // KO.STATE8_BLOCK, -(-own.stop // KO.STATE8_BLOCK))
+        h = self.hyper(step)
+        h.pop('l2')
+        KO.adamw8(param, grad, flat.s1[own], flat.s2[own], flat.s1_scale[blocks], flat.s2_scale[blocks], shadow,
+                  gscale=flat.gscale, seed=seed, dyn=dyn, **h)
+
+    def dense_update(self, flat, step, dyn=None):
+        if self.state_bits == 32:
+            return super().dense_update(flat, step, dyn)
+        self._update8(flat, flat.param, flat.grad, slice(0, flat.param.numel()), flat.shadow, step, dyn)
+
+    def shard_update(self, flat, lo, hi, own, step, dyn=None):
+        if self.state_bits == 32:
+            return super().shard_update(flat, lo, hi, own, step, dyn)
+        self._update8(flat, flat.param[lo:hi], flat.zgrad[own], own, None, step, dyn)
 
 
 class LambOptimizer(AdamWOptimizer):
@@ -181,11 +219,11 @@ class LambOptimizer(AdamWOptimizer):
 SEG_ALIGN = 8   # flat-buffer segment alignment in elements (FlatGroup)
 
 
-def flat_extent(numels):
-    """elements a FlatGroup of segments of these sizes spans (SEG_ALIGN-aligned starts)"""
+def flat_extent(numels, align=SEG_ALIGN):
+    """elements a FlatGroup of segments of these sizes spans (aligned starts)"""
     off = 0
     for n in numels:
-        off = -(-off // SEG_ALIGN) * SEG_ALIGN + n
+        off = -(-off // align) * align + n
     return off
 
 
@@ -205,15 +243,18 @@ class FlatGroup(object):
 
     def __init__(self, params: List[Op], values: Dict[Op, torch.Tensor], n_states: int,
                  state_init=(0.0, 0.0), shadow: bool = False, device=None, pad_to: int = 1,
-                 state_numel: Optional[int] = None):
+                 state_numel: Optional[int] = None, state_bits: int = 32):
         self.params = params
+        self.state_bits = state_bits
+        # 8-bit moments share a scale over blocks of 256: no block reaches into two parameters
+        self.align = SEG_ALIGN if state_bits == 32 else KO.STATE8_BLOCK
         self.offsets = {}
         off = 0
         for p in params:
             # every segment starts 16-byte aligned in the bf16 shadow (8 elements): the
             # MFMA loaders stage 16-byte chunks, and one odd-sized bias ahead of a weight
             # (the MoE gate's 2) otherwise sent every later weight to the library GEMM
-            off = -(-off // SEG_ALIGN) * SEG_ALIGN
+            off = -(-off // self.align) * self.align
             self.offsets[p] = (off, values[p].numel(), tuple(values[p].shape))
             off += values[p].numel()
         self.numel = off
@@ -225,8 +266,13 @@ class FlatGroup(object):
             self.view(p, 'param').copy_(values[p].float())
         self.grad = _NA.zeros_like(self.param)
         ns = self.padded if state_numel is None else state_numel   # ZeRO-1: this rank's shard only
-        self.s1 = _filled((ns,), state_init[0], dev) if n_states >= 1 else None
-        self.s2 = _filled((ns,), state_init[1], dev) if n_states >= 2 else None
+        self.s1_scale = self.s2_scale = None
+        self.rng_key = 0
+        if state_bits == 8:
+            self.s1, self.s2, self.s1_scale, self.s2_scale = KO.adamw8_state(ns, dev)
+        else:
+            self.s1 = _filled((ns,), state_init[0], dev) if n_states >= 1 else None
+            self.s2 = _filled((ns,), state_init[1], dev) if n_states >= 2 else None
         self.shadow = None
         if shadow:
             self.shadow = self.param.to(torch.bfloat16)  # same (channels-last) layout
@@ -361,13 +407,16 @@ class OptimizerOp(Op):
         pad_to, state_numel = 1, None
         if self.zero:
             P = self.comm.nrank
-            self.zero_unit = P * 64                       # every bucket splits into 64-aligned shards
+            # every bucket splits into 64-aligned shards (of whole blocks of 8-bit moments)
+            align = SEG_ALIGN if opt.state_bits == 32 else KO.STATE8_BLOCK
+            self.zero_unit = P * max(64, align)
             pad_to = self.zero_unit
-            total = -(-flat_extent([values[p].numel() for p in dense]) // pad_to) * pad_to
+            total = -(-flat_extent([values[p].numel() for p in dense], align) // pad_to) * pad_to
             state_numel = max(total // P, 1)
         self.flat = FlatGroup(dense, values, opt.n_states, getattr(opt, 'state_init', (0.0, 0.0)),
                               shadow=amp, device=self.ctx.torch_device if self.ctx else None,
-                              pad_to=pad_to, state_numel=state_numel)
+                              pad_to=pad_to, state_numel=state_numel, state_bits=opt.state_bits)
+        self.flat.rng_key = self.id
         # ops that can write their gradient straight into the flat buffer get its view
         grad_of = {pp: g for pp, g in zip(self.param_of_input, self.inputs)}
         for p in dense:
@@ -400,6 +449,9 @@ class OptimizerOp(Op):
         elif self.dp:
             self._make_buckets(dense)
         if self.ps_dense_wanted and self.flat.numel > 0:
+            if opt.state_bits != 32:
+                raise ValueError('%s(state_bits=%d): the parameter server holds the dense state (comm_mode PS)'
+                                 % (type(opt).__name__, opt.state_bits))
             from .ps.table import PSDense
             from .ps import PS_KEY_OPT_FLAT
             # key space: node ids are < 2^20; the flat dense key sits above them
@@ -414,11 +466,12 @@ class OptimizerOp(Op):
         full = max(self.bucket_bytes // 4, 1)
         cap = max(full // 8, 1)
         groups, cur, cur_n, nxt = [], [], 0, None
+        align = getattr(self.flat, 'align', SEG_ALIGN)
         for p in reversed([p for p in dense if not self.excluded_from_dp(p)]):
             o, n, _ = self.flat.offsets[p]
             # members must stay contiguous in the flat buffer (the next member starts at
             # the aligned end of this one; the alignment gap rides along, all zeros)
-            if cur and (-(-(o + n) // SEG_ALIGN) * SEG_ALIGN != nxt or cur_n + n > cap):
+            if cur and (-(-(o + n) // align) * align != nxt or cur_n + n > cap):
                 groups.append(cur)
                 cur, cur_n = [], 0
                 cap = min(cap * 2, full)
@@ -489,7 +542,6 @@ class OptimizerOp(Op):
 
     def _zero_step(self):
         f, opt = self.flat, self.optimizer
-        h = opt.hyper(self.step)
         dyn = getattr(self, 'dyn', None)
         gathers = []
         for b in self.buckets:
@@ -498,9 +550,7 @@ class OptimizerOp(Op):
             else:
                 self._reduce_bucket(b, async_op=False)
             lo, hi = b.own
-            sl = slice(b.zoff, b.zoff + hi - lo)
-            KO.optimizer_flat(opt.mode, f.param[lo:hi], f.zgrad[sl], f.s1[sl] if f.s1 is not None else None,
-                              f.s2[sl] if f.s2 is not None else None, None, gscale=f.gscale, dyn=dyn, **h)
+            opt.shard_update(f, lo, hi, slice(b.zoff, b.zoff + hi - lo), self.step, dyn)
             # the gather of this bucket overlaps the update of the next one
             gathers.append(self.comm.all_gather(f.param[b.start:b.end], f.param[lo:hi].clone(), async_op=True))
         for w in gathers:

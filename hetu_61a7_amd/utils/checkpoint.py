@@ -161,6 +161,73 @@ def _ps_save(ex, file_path):
     agent.BarrierWorker()
 
 
+def _moments(fl):
+    """a flat buffer's moments as arrays: fp32 ``s1`` / ``s2``, or the bytes of 8-bit moments with
+    their blocks' scales"""
+    d = {k: None if getattr(fl, k) is None else getattr(fl, k).cpu() for k in ('s1', 's2')}
+    if getattr(fl, 'state_bits', 32) == 8:
+        d = {k: t.view(torch.uint8) for k, t in d.items()}
+        d.update(s1_scale=fl.s1_scale.cpu(), s2_scale=fl.s2_scale.cpu())
+    return {k: None if t is None else t.numpy() for k, t in d.items()}
+
+
+_STATE8 = {'s1': torch.float8_e4m3fn, 's2': torch.float8_e5m2}
+
+
+def _fp32_moments(d):
+    """record ``d`` with 8-bit moments read as the fp32 values they stand for"""
+    if d.get('s1_scale') is None:
+        return d
+    from ..kernels.optim import state8_values
+    d = dict(d)
+    for k, dt in _STATE8.items():
+        d[k] = state8_values(torch.from_numpy(np.array(d[k])).view(dt), torch.from_numpy(np.array(d.pop(k + '_scale')))).numpy()
+    return d
+
+
+def _set_moment(fl, k, values):
+    """the whole moment ``k`` of a flat buffer from fp32 ``values`` (an array)"""
+    buf = getattr(fl, k)
+    t = torch.from_numpy(np.ascontiguousarray(values, dtype=np.float32))
+    if getattr(fl, 'state_bits', 32) == 8:
+        from ..kernels.optim import state8_from_values
+        q, scale = state8_from_values(t, k)
+        buf.view(torch.uint8).copy_(q.view(torch.uint8))
+        getattr(fl, k + '_scale').copy_(scale)
+    else:
+        buf.copy_(t.to(buf.device))
+
+
+def _set_moments_as_saved(fl, d):
+    """the moments of a record of the same layout and form, bit by bit; False: another form"""
+    if (d.get('s1_scale') is not None) != (getattr(fl, 'state_bits', 32) == 8) or d.get('s1_scale') is None:
+        return False
+    for k in _STATE8:
+        getattr(fl, k).view(torch.uint8).copy_(torch.from_numpy(np.array(d[k])))
+        getattr(fl, k + '_scale').copy_(torch.from_numpy(np.array(d[k + '_scale'])))
+    return True
+
+
+def _relaid(fl, d):
+    """a whole-buffer record with 8-bit moments on either side, as fp32 moments in this buffer's
+    layout (its segments start at other offsets than those of a buffer with 32-bit moments)"""
+    if d.get('zero') or d.get('layout') is None or d.get('s1') is None or \
+            (d.get('s1_scale') is None and getattr(fl, 'state_bits', 32) == 32):
+        return d
+    d = dict(_fp32_moments(d))
+    saved = {name: (o, n) for name, o, n in d['layout']}
+    for k in _STATE8:
+        full = np.zeros(fl.padded, np.float32)
+        for p in fl.params:
+            o, n, _ = fl.offsets[p]
+            so, sn = saved.get(p.name, (0, 0))
+            if sn not in (0, n):
+                raise ValueError('parameter %s has %d elements, the checkpoint %d' % (p.name, n, sn))
+            full[o:o + sn] = np.asarray(d[k]).reshape(-1)[so:so + sn]
+        d[k] = full
+    return d
+
+
 def _ext_state(ex, zero_rank):
     ext = {'optimizers': [], 'bn': {}}
     for op in _opt_ops(ex):
@@ -172,8 +239,7 @@ def _ext_state(ex, zero_rank):
             # (optimizer.SEG_ALIGN) and the parameter set may differ at load time
             d['layout'] = [(p.name, int(fl.offsets[p][0]), int(fl.offsets[p][1])) for p in fl.params]
             if not d['zero']:   # ZeRO shards go to the per-rank file
-                d['s1'] = fl.s1.cpu().numpy() if fl.s1 is not None else None
-                d['s2'] = fl.s2.cpu().numpy() if fl.s2 is not None else None
+                d.update(_moments(fl))
         d['sparse'] = {p.name: {k: v.detach().float().cpu().numpy() for k, v in st.items()}
                        for p, st in op.sparse_state.items()}
         lr = op.optimizer.learning_rate
@@ -194,9 +260,7 @@ def _zero_shards(ex):
         if not getattr(op, 'zero', False) or fl is None:
             out.append(None)
             continue
-        out.append({'s1': fl.s1.cpu().numpy() if fl.s1 is not None else None,
-                    's2': fl.s2.cpu().numpy() if fl.s2 is not None else None,
-                    'nrank': op.comm.nrank, 'rank': op.comm.rank})
+        out.append(dict(_moments(fl), nrank=op.comm.nrank, rank=op.comm.rank))
     return out
 
 
@@ -303,6 +367,10 @@ def _load_flat_moments(fl, d, i):
     than loaded under the wrong offsets."""
     import numpy as np
     layout = d.get('layout')
+    if layout is not None and layout == [(p.name, int(fl.offsets[p][0]), int(fl.offsets[p][1])) for p in fl.params] \
+            and _set_moments_as_saved(fl, d):
+        return
+    d = _fp32_moments(d)
     for k in ('s1', 's2'):
         buf = getattr(fl, k)
         arr = d.get(k)
@@ -317,10 +385,14 @@ def _load_flat_moments(fl, d, i):
                                  're-save the checkpoint with this version' %
                                  (i, arr.size, buf.numel(), 'matches' if order == [p.name for p in fl.params]
                                   else 'differs'))
-            buf.copy_(torch.from_numpy(arr).to(buf.device))
+            _set_moment(fl, k, arr)
             continue
         saved = {name: (o, n) for name, o, n in layout}
-        host = buf.detach().cpu().numpy().copy()
+        if getattr(fl, 'state_bits', 32) == 8:
+            from ..kernels.optim import state8_values
+            host = state8_values(buf, getattr(fl, k + '_scale')).cpu().numpy().copy()
+        else:
+            host = buf.detach().cpu().numpy().copy()
         for p in fl.params:
             o, n, _ = fl.offsets[p]
             if p.name not in saved:
@@ -330,7 +402,7 @@ def _load_flat_moments(fl, d, i):
                 raise ValueError('optimizer %d: parameter %s has %d elements, the checkpoint %d'
                                  % (i, p.name, n, sn))
             host[o:o + n] = arr[so:so + sn]
-        buf.copy_(torch.from_numpy(host).to(buf.device))
+        _set_moment(fl, k, host)
 
 
 def load(ex, file_path, file_name='checkpoint.pkl', consider_splits=False):
@@ -352,6 +424,8 @@ def load(ex, file_path, file_name='checkpoint.pkl', consider_splits=False):
         op.step = d['step']
         fl = op.flat
         src = d
+        if getattr(op, 'zero', False) and fl is not None:
+            src = d = _relaid(fl, d)
         if getattr(op, 'zero', False):
             if shards is None or i >= len(shards) or shards[i] is None:
                 if _full_moments(d, fl, op):
@@ -372,10 +446,11 @@ def load(ex, file_path, file_name='checkpoint.pkl', consider_splits=False):
             if src is d:
                 _load_flat_moments(fl, d, i)
             else:
-                for k in ('s1', 's2'):
-                    buf = getattr(fl, k)
-                    if src.get(k) is not None and buf is not None:
-                        buf.copy_(torch.from_numpy(src[k]).to(buf.device))
+                if not _set_moments_as_saved(fl, src):
+                    src = _fp32_moments(src)
+                    for k in ('s1', 's2'):
+                        if src.get(k) is not None and getattr(fl, k) is not None:
+                            _set_moment(fl, k, src[k])
         by_name = {p.name: st for p, st in op.sparse_state.items()}
         for name, st in d.get('sparse', {}).items():
             if name in by_name:

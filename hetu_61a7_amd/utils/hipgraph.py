@@ -119,14 +119,18 @@ class GraphRunner(object):
         for op in self.sub.opt_ops:
             opt = op.optimizer
             if getattr(op, 'dyn', None) is None:
-                op.dyn = _NA.zeros(4, dtype=torch.float32, device=self.sub.config.device)
-                op.dyn_host = _NA.zeros(4, dtype=torch.float32).pin_memory()
+                # lr, beta1^t, beta2^t, gradient scale, step, 1 - beta1^t, 1 - beta2^t
+                op.dyn = _NA.zeros(7, dtype=torch.float32, device=self.sub.config.device)
+                op.dyn_host = _NA.zeros(7, dtype=torch.float32).pin_memory()
             step = op.step + 1
             h = opt.hyper(step)
             op.dyn_host[0] = h.get('lr', 0.0)
             op.dyn_host[1] = h.get('beta1t', 1.0)
             op.dyn_host[2] = h.get('beta2t', 1.0)
             op.dyn_host[3] = op.flat.gscale if op.flat is not None else 1.0
+            op.dyn_host[4] = step
+            op.dyn_host[5] = 1.0 - h.get('beta1t', 1.0)
+            op.dyn_host[6] = 1.0 - h.get('beta2t', 1.0)
             op.dyn.copy_(op.dyn_host, non_blocking=True)
 
     def run(self, feed_dict, convert):

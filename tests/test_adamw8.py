@@ -1,0 +1,306 @@
+"""AdamW with 8-bit moments: the CPU form and the HIP kernel against the definition in 64 bits, and
+the optimizer that uses it."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import hetu_61a7_amd as ht
+from hetu_61a7_amd.kernels import optim as KO
+
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+U = 2.0 ** -24                      # half a unit of fp32
+FORMS = {'m': (7, 3, -6), 'v': (14, 2, -14)}     # largest exponent in a block, mantissa bits, least exponent
+
+
+def _inputs(n, seed, device, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    size = 1e-3 * torch.exp(spread * torch.randn(n, generator=g))
+    p = 0.05 * torch.randn(n, generator=g)
+    grad = size * torch.randn(n, generator=g)
+    m, v, ms, vs = KO.adamw8_state(n, 'cpu')
+    for q, s, x, k in ((m, ms, 0.3 * size * torch.randn(n, generator=g), 's1'),
+                       (v, vs, size.square() * torch.rand(n, generator=g), 's2')):
+        a, b = KO.state8_from_values(x, k)
+        q.view(torch.uint8).copy_(a.view(torch.uint8))
+        s.copy_(b)
+    return [t.to(device) for t in (p, grad, m, v, ms, vs)]
+
+
+def _definition(p, g, m, v, ms, vs, h):
+    """(p', m', v') in 64 bits"""
+    p, g = p.double(), g.double() * h.get('gscale', 1.0)
+    block = torch.arange(p.numel(), device=p.device) // 256
+    m = h['beta1'] * m.double() * ms.double()[block] + (1 - h['beta1']) * g
+    v = h['beta2'] * v.double() * vs.double()[block] + (1 - h['beta2']) * g ** 2
+    u = m / (1 - h['beta1t']) / ((v / (1 - h['beta2t'])).sqrt() + h['eps'])
+    return p - h['lr'] * (u + h['wd'] * p), m, v
+
+
+def _check_state(name, x, q, scale):
+    """q * scale is one of the two grid values around ``x`` (fp32 roundings of x allowed for), on
+    the grid that the block's largest value sets"""
+    top, mant, least = FORMS[name]
+    n = x.numel()
+    block = torch.arange(n, device=x.device) // 256
+    most = torch.zeros(scale.numel(), dtype=torch.float64, device=x.device).scatter_reduce_(0, block, x.abs(), 'amax')
+    want = torch.exp2((torch.frexp(most)[1] - 1 - top).clamp_min(-126).double())
+    near = (torch.frexp(most * (1 + 8 * U))[1] != torch.frexp(most * (1 - 8 * U))[1])   # on a binade's border
+    assert bool(((scale.double() == want) | near).all())
+    s = scale.double()[block]
+    y = x.abs() / s
+    step = torch.exp2((torch.frexp(y)[1] - 1).clamp_min(least).double() - mant)
+    got = q.double().abs()
+    # x' has three roundings of its terms: 3 U of |beta m| + |(1 - beta) g| <= 8 U of the block's largest
+    slack = 8 * U * (y + torch.exp2(torch.tensor(float(top + 1), dtype=torch.float64)))
+    assert bool(((got - y).abs() <= step + slack).all())
+    assert bool((got / step == torch.round(got / step)).all())
+    if name == 'v':
+        assert bool((got[x > 0] > 0).all())
+    else:
+        assert bool((torch.signbit(q.float()) == (x < 0))[y > slack].all())
+
+
+H = dict(lr=1e-3, beta1=0.9, beta2=0.999, beta1t=0.9 ** 7, beta2t=0.999 ** 7, eps=1e-7, wd=0.01)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('shadow', [False, True])
+@pytest.mark.parametrize('n', [1, 3, 4, 255, 256, 257, 1000, 4099, 70001])
+def test_step_matches_definition(n, shadow, device):
+    p, g, m, v, ms, vs = _inputs(n, n, device)
+    ref, m64, v64 = _definition(p, g, m, v, ms, vs, H)
+    p0, sh = p.clone(), torch.zeros(n, dtype=torch.bfloat16, device=device) if shadow else None
+    KO.adamw8(p, g, m, v, ms, vs, sh, seed=n * 17, **H)
+    # u = mhat / (sqrt(vhat) + eps): about 10 roundings, p's own two.  m' itself cancels: its error is
+    # 3 U of its terms, which reach u through 1 / sqrt(vhat); |terms| <= |m'| + 2 * 0.1 |g|
+    unit = (m64.abs() + 0.2 * g.double().abs()) / (1 - H['beta1t']) / ((v64 / (1 - H['beta2t'])).sqrt() + H['eps'])
+    tol = 2 * U * p0.double().abs() + H['lr'] * 16 * U * (unit + H['wd'] * p0.double().abs()) + U * ref.abs()
+    assert bool(((p.double() - ref).abs() <= tol).all())
+    _check_state('m', m64, m, ms)
+    _check_state('v', v64, v, vs)
+    if shadow:
+        assert torch.equal(sh, p.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 257, 4099, 1 << 18])
+def test_kernel_stores_the_cpu_forms_bits(n):
+    """the moments are rounded operation by operation: the kernel and plain fp32 arithmetic agree bit by bit"""
+    a, b = _inputs(n, n + 1, 'cpu'), _inputs(n, n + 1, 'cuda')
+    for step in range(3):
+        for s in (a, b):
+            KO.adamw8(*s, seed=KO.step_seed(n, step), gscale=0.5, **H)
+    for x, y in zip(a[2:], b[2:]):
+        assert torch.equal(x.view(torch.uint8), y.cpu().view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_unaligned_slices():
+    n = 1000
+    whole = [torch.zeros(n + 8, dtype=t.dtype, device='cuda') if t.numel() == n else t for t in _inputs(n, 3, 'cuda')]
+    sh = torch.zeros(n + 8, dtype=torch.bfloat16, device='cuda')
+    for off in (1, 2, 3):
+        src = _inputs(n, 3, 'cuda')
+        part = [w[off:off + n] if w.numel() == n + 8 else s.clone() for w, s in zip(whole, src)]   # (the scales: their own)
+        for d, s in zip(part, src):
+            d.view(torch.uint8).copy_(s.view(torch.uint8))
+        KO.adamw8(*src, seed=9, **H)
+        KO.adamw8(*part, sh[off:off + n], seed=9, **H)
+        for x, y in zip(src, part):
+            assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))
+        assert torch.equal(sh[off:off + n], part[0].to(torch.bfloat16))
+        for w in whole + [sh]:
+            if w.numel() == n + 8:
+                assert float(w[:off].float().abs().sum()) == 0 and float(w[off + n:].float().abs().sum()) == 0
+                w.zero_()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_rounding_has_no_bias(device):
+    """N equal values between two grid values: their stored mean is the value, within 6 standard
+    errors of a two-valued variable (at most half a step each) and the 2^-17 of a step that 16
+    random bits resolve"""
+    N = 256 * 512
+    p, g, m, v, ms, vs = _inputs(N, 0, device)
+    for t in (m, v):
+        t.view(torch.uint8).zero_()
+    g.fill_(0.37)
+    g[::256] = 1.0                      # the blocks' largest: the others lie below the top binade
+    KO.adamw8(p, g, m, v, ms, vs, seed=5, **H)
+    pick = torch.arange(N, device=device) % 256 != 0
+    for q, s, x, (top, mant, least) in ((m, ms, 0.1 * 0.37, FORMS['m']), (v, vs, 0.001 * 0.37 ** 2, FORMS['v'])):
+        got = KO.state8_values(q, s)[pick].double()
+        step = 2.0 ** (math.floor(math.log2(x)) - mant)
+        assert len(got.unique()) == 2
+        assert abs(float(got.mean()) - x) <= step * (3 / math.sqrt(int(pick.sum())) + 2.0 ** -17) + 8 * U * x
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_other_seeds_round_differently(device):
+    runs = []
+    for seed in (1, 2, 1, (1 << 64) - 1, 1 << 40):
+        s = _inputs(5000, 4, device)
+        KO.adamw8(*s, seed=seed, **H)
+        runs.append(s[2].view(torch.uint8).clone())
+    assert torch.equal(runs[0], runs[2])
+    # an element rounds the other way with probability 2 f (1 - f), a third on average
+    for other in (runs[1], runs[3], runs[4]):
+        assert 0.2 < float((runs[0] != other).float().mean()) < 0.45
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_not_finite_gradients_stay_with_their_elements(device):
+    n = 600
+    s = _inputs(n, 6, device)
+    clean = [t.clone() for t in s]
+    for t in (s, clean):
+        t[1][17], t[1][300], t[1][301] = 0.0, 0.0, 0.0
+        t[2].view(torch.uint8)[[17, 300, 301]] = 0
+    s[1][17], s[1][300], s[1][301] = float('nan'), float('inf'), -float('inf')
+    KO.adamw8(*s, seed=8, **H)
+    KO.adamw8(*clean, seed=8, **H)
+    rest = torch.ones(n, dtype=torch.bool, device=device)
+    rest[[17, 300, 301]] = False
+    for x, y in zip((s[0], s[2], s[3]), (clean[0], clean[2], clean[3])):
+        assert torch.equal(x.view(-1, 1).view(torch.uint8).view(n, -1)[rest], y.view(-1, 1).view(torch.uint8).view(n, -1)[rest])
+    assert torch.equal(s[4], clean[4]) and torch.equal(s[5], clean[5])
+    assert bool(s[0][[17, 300, 301]].isnan().all())
+    assert bool(s[2].float()[[17, 300, 301]].isnan().all())
+    assert bool(s[3].float()[17].isnan()) and bool(s[3].float()[[300, 301]].isinf().all())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_zero_and_tiny(device):
+    """nothing to step on stays as it is; values below the normal range keep a scale that is normal"""
+    n = 520
+    p, g, m, v, ms, vs = [t.to(device) for t in (torch.randn(n), torch.zeros(n)) + tuple(KO.adamw8_state(n, 'cpu'))]
+    p0 = p.clone()
+    KO.adamw8(p, g, m, v, ms, vs, seed=1, **dict(H, wd=0.0))
+    assert torch.equal(p, p0) and not m.view(torch.uint8).any() and not v.view(torch.uint8).any()
+    assert bool((ms == 2.0 ** -126).all()) and bool((vs == 2.0 ** -126).all())
+    g.fill_(1e-30)
+    KO.adamw8(p, g, m, v, ms, vs, seed=1, **dict(H, wd=0.0))
+    assert bool(torch.isfinite(p).all()) and bool(torch.isfinite(KO.state8_values(m, ms)).all())
+
+
+def test_refusals():
+    s = _inputs(300, 1, 'cpu')
+    bad = [(0, s[0].double()), (1, s[1][:299]), (2, s[2].view(torch.uint8)), (3, s[3].view(torch.float8_e4m3fn)),
+           (4, s[4][:1]), (5, s[5].double()), (0, torch.zeros(600)[::2])]
+    for i, t in bad:
+        with pytest.raises(ValueError):
+            KO.adamw8(*[t if j == i else x for j, x in enumerate(s)], **H)
+    with pytest.raises(ValueError):
+        KO.adamw8(*s, torch.zeros(300), **H)
+    with pytest.raises(ValueError):
+        KO.adamw8(*s, dyn=torch.zeros(4), **H)
+    with pytest.raises(ValueError):
+        ht.optim.AdamWOptimizer(state_bits=4)
+    KO.adamw8(*[t[:0] for t in s], **H)                     # no elements: nothing to do
+
+
+# ---- through the optimizer ---------------------------------------------------------------------
+def _net(bits, rng, lr=0.01):
+    x, y_ = ht.Variable(name='x'), ht.Variable(name='y_')
+    w1 = ht.Variable(name='w1', value=(rng.randn(20, 33) * 0.3).astype(np.float32))
+    b1 = ht.Variable(name='b1', value=np.zeros(33, np.float32))
+    w2 = ht.Variable(name='w2', value=(rng.randn(33, 5) * 0.3).astype(np.float32))
+    h = ht.relu_op(ht.linear_op(x, w1, b1))
+    loss = ht.reduce_mean_op(ht.softmaxcrossentropy_op(ht.matmul_op(h, w2), y_), [0])
+    train = ht.optim.AdamWOptimizer(lr, weight_decay=0.01, state_bits=bits).minimize(loss)
+    return x, y_, loss, train
+
+
+def _feed(rng, x, y_, rows=16):
+    return {x: rng.randn(rows, 20).astype(np.float32), y_: np.eye(5, dtype=np.float32)[rng.randint(0, 5, rows)]}
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_optimizer_first_step_and_layout(device):
+    """the first step has no stored moments: it equals the 32-bit optimizer's, and every
+    parameter's block of state is its own"""
+    ctx = ht.cpu(0) if device == 'cpu' else ht.gpu(0)
+    got = {}
+    for bits in (8, 32):
+        rng = np.random.RandomState(0)
+        x, y_, loss, train = _net(bits, rng)
+        ex = ht.Executor({'train': [loss, train]}, ctx=ctx, seed=3)
+        ex.run('train', feed_dict=_feed(rng, x, y_))
+        got[bits] = {n.name: v.float().cpu() for n, v in ex.config.placeholder_to_arr_map.items() if n.trainable}
+        if bits == 8:
+            f = train.flat
+            assert f.s1.dtype == torch.float8_e4m3fn and f.s2.dtype == torch.float8_e5m2
+            assert all(f.offsets[p][0] % 256 == 0 for p in f.params)
+    for k in got[8]:
+        # the update is at most lr * (1 + wd |p|), computed in two orders: 32 roundings of it
+        torch.testing.assert_close(got[8][k], got[32][k], rtol=4 * U, atol=32 * U * 0.02)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_checkpoint_resumes_bit_by_bit(tmp_path, device):
+    """weights, 8-bit moments and the rounding's seeds come back: a resumed run takes the steps of
+    one that was not interrupted; 32-bit moments load into 8 bits and back by their values"""
+    ctx = ht.cpu(0) if device == 'cpu' else ht.gpu(0)
+
+    def make(bits):
+        rng = np.random.RandomState(1)
+        x, y_, loss, train = _net(bits, rng)
+        return ht.Executor({'train': [loss, train]}, ctx=ctx, seed=3, use_hipgraph=False), x, y_, train
+
+    def steps(ex, x, y_, a, b):
+        for i in range(a, b):
+            ex.run('train', feed_dict=_feed(np.random.RandomState(100 + i), x, y_))
+
+    ex, x, y_, train = make(8)
+    steps(ex, x, y_, 0, 3)
+    ex.save(str(tmp_path), save_optimizer=True)
+    steps(ex, x, y_, 3, 6)
+    ex2, x2, y2, train2 = make(8)
+    ex2.load(str(tmp_path))
+    # parameters are found by name; node ids differ between the two graphs and with them the seeds
+    train2.flat.rng_key = train.flat.rng_key
+    steps(ex2, x2, y2, 3, 6)
+    for a, b in ((train.flat.param, train2.flat.param), (train.flat.s1, train2.flat.s1), (train.flat.s2, train2.flat.s2),
+                 (train.flat.s1_scale, train2.flat.s1_scale)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    ex3, _, _, train3 = make(32)
+    ex3.load(str(tmp_path))
+    ex4, _, _, train4 = make(8)
+    ex4.load(str(tmp_path))
+    ex3.save(str(tmp_path / 'wide'), save_optimizer=True)
+    ex5, _, _, train5 = make(8)
+    ex5.load(str(tmp_path / 'wide'))
+    for k in ('s1', 's2'):
+        v = [KO.state8_values(getattr(t.flat, k), getattr(t.flat, k + '_scale')) for t in (train4, train5)]
+        flat = getattr(train3.flat, k)
+        for p4, p3, p5 in zip(train4.flat.params, train3.flat.params, train5.flat.params):
+            o, n, _ = train4.flat.offsets[p4]
+            o3 = train3.flat.offsets[p3][0]
+            assert torch.equal(v[0][o:o + n], flat[o3:o3 + n])
+            # written again: a block whose largest value was rounded into the next binade gets a
+            # grid twice as wide, half a step of which is 2^-4 (e4m3) or 2^-3 (e5m2) of a value
+            half = 2.0 ** -4 if k == 's1' else 2.0 ** -3
+            least = (2.0 ** -10 if k == 's1' else 2.0 ** -16) * getattr(train5.flat, k + '_scale').max()
+            assert bool(((v[1][o:o + n] - flat[o3:o3 + n]).abs() <= half * flat[o3:o3 + n].abs() + least).all())
+
+
+@pytest.mark.gpu
+def test_replayed_steps_equal_eager_ones():
+    """a captured step takes its step number, rates and rounding seed from device memory"""
+    runs = []
+    for graph in (False, True):
+        rng = np.random.RandomState(2)
+        x, y_, loss, train = _net(8, rng)
+        ex = ht.Executor({'train': [loss, train]}, ctx=ht.gpu(0), seed=3, use_hipgraph=graph)
+        train.flat.rng_key = 77
+        feed = _feed(rng, x, y_)
+        for i in range(8):
+            ex.run('train', feed_dict=feed)
+            torch.cuda.synchronize()
+            torch.randn(1000, device='cuda').sum().item()      # the program's own work in between
+        runs.append([train.flat.param.clone(), train.flat.s1.view(torch.uint8).clone(), train.flat.s2.view(torch.uint8).clone()])
+        assert train.step == 8
+    for a, b in zip(*runs):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
