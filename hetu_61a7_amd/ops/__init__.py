@@ -38,7 +38,7 @@ from .loss import (softmax_func, softmax_op, softmax_gradient_op, softmaxcrossen
                    softmaxcrossentropy_sparse_gradient_op, crossentropy_op,
                    crossentropy_gradient_op, crossentropy_sparse_op,
                    crossentropy_sparse_gradient_op, binarycrossentropy_op,
-                   binarycrossentropy_gradient_op, nll_loss_op, nll_loss_grad_op)
+                   binarycrossentropy_gradient_op, nll_loss_op, nll_loss_grad_op, token_logprob_op)
 from .embedding import embedding_lookup_op, embedding_lookup_gradient_op
 from .transfer import datah2d_op, datad2h_op, datah2d_sparse_op, datad2h_sparse_op
 from .comm import (allreduceCommunicate_op, allreduceCommunicatep2p_op,

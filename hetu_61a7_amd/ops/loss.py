@@ -366,3 +366,124 @@ def nll_loss_op(input, target, cols, ctx=None):
 
 def nll_loss_grad_op(output_grad, target, cols, ref=None, ctx=None):
     return NllLossGradOp(output_grad, target, cols, ref, ctx=ctx)
+
+
+# ---------------------------------------------------------------------------
+# Log probabilities of given tokens, entropy and alternatives (kernels/logprob.py): one op whose
+# value holds all columns [..., 2 + top], so that the gradients of every column join in that small
+# tensor and the logits' gradient is one pass.
+class TokenLogProbOp(Op):
+    def __init__(self, logits, ids, top=0, ignored_index=-1, ctx=None):
+        super().__init__(TokenLogProbOp, [logits, ids], ctx)
+        _label_feed(ids)
+        self.top, self.ignored_index = int(top), int(ignored_index)
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        from ..kernels import logprob as KL
+        r = KL.token_logprob(input_vals[0], input_vals[1], self.top, self.ignored_index)
+        return AuxResult(r.out, r)
+
+    def gradient(self, output_grad):
+        return [TokenLogProbGradientOp(output_grad, self, ctx=self.raw_ctx), None]
+
+    def infer_shape(self, input_shapes):
+        return tuple(input_shapes[0][:-1]) + (2 + self.top,)
+
+
+class TokenLogProbGradientOp(Op):
+    aux_inputs = (3,)
+
+    def __init__(self, grad, fwd, ctx=None):
+        super().__init__(TokenLogProbGradientOp, [fwd.inputs[0], fwd.inputs[1], grad, fwd], ctx)
+        self.ignored_index = fwd.ignored_index
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        from ..kernels import logprob as KL
+        x, ids, g, r = input_vals
+        return KL.token_logprob_backward(x, ids, r, g, self.ignored_index)
+
+    def gradient(self, output_grad):
+        raise NotImplementedError
+
+    def infer_shape(self, input_shapes):
+        return input_shapes[0]
+
+
+class TokenLogProbPickOp(Op):
+    """columns [begin, begin + size) of the op above; size 0: the one column, without its axis"""
+
+    def __init__(self, node, begin, size=0, ctx=None):
+        super().__init__(TokenLogProbPickOp, [node], ctx)
+        self.begin, self.size = begin, size
+
+    def _pick(self, t):
+        return t[..., self.begin] if self.size == 0 else t[..., self.begin:self.begin + self.size]
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        v = self._pick(input_vals[0])
+        if v.is_cuda:
+            return KT.copy_into(_NA.empty(tuple(v.shape), dtype=v.dtype, device=v.device), v)
+        return v.clone()
+
+    def gradient(self, output_grad):
+        return [TokenLogProbPickGradientOp(output_grad, self, ctx=self.raw_ctx)]
+
+    def infer_shape(self, input_shapes):
+        return tuple(input_shapes[0][:-1]) + ((self.size,) if self.size else ())
+
+
+class TokenLogProbPickGradientOp(Op):
+    shape_only_inputs = (1,)
+
+    def __init__(self, grad, pick, ctx=None):
+        super().__init__(TokenLogProbPickGradientOp, [grad, pick.inputs[0]], ctx)
+        self.pick = pick
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        g, shape = input_vals
+        out = _NA.zeros(tuple(shape), dtype=torch.float32, device=g.device)
+        dst = self.pick._pick(out)
+        if g.shape != dst.shape:
+            g = g.expand(dst.shape) if g.numel() == 1 else g.reshape(dst.shape)
+        if g.dtype != torch.float32:
+            g = g.float()
+        if g.is_cuda:
+            KT.copy_into(dst, g)
+        else:
+            dst.copy_(g)
+        return out
+
+    def gradient(self, output_grad):
+        raise NotImplementedError
+
+    def infer_shape(self, input_shapes):
+        return input_shapes[1]
+
+
+class TokenLogProbIdsOp(Op):
+    aux_inputs = (0,)
+
+    def __init__(self, node, ctx=None):
+        super().__init__(TokenLogProbIdsOp, [node], ctx)
+        self.top = node.top
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        return input_vals[0].top_ids
+
+    def gradient(self, output_grad):
+        return [None]
+
+    def infer_shape(self, input_shapes):
+        return tuple(input_shapes[0][:-1]) + (self.top,)
+
+
+def token_logprob_op(logits, ids, top=0, ignored_index=-1, ctx=None):
+    """(logp [...], entropy [...]) of token ``ids`` [...] under ``logits`` [..., V], in nats, fp32;
+    with ``top`` > 0 also (top_logp [..., top], top_ids [..., top]): the most probable tokens.  All
+    but the ids are differentiable with respect to the logits.  A row whose id is ``ignored_index``
+    or outside [0, V) is 0 in all (ids -1) and gets no gradient (``kernels.logprob``)."""
+    if not 0 <= int(top) <= 64:
+        raise ValueError('token_logprob_op: top is 0 to 64, got %r' % (top,))
+    n = TokenLogProbOp(logits, ids, top, ignored_index, ctx=ctx)
+    r = (TokenLogProbPickOp(n, 0, ctx=ctx), TokenLogProbPickOp(n, 1, ctx=ctx))
+    return r + (TokenLogProbPickOp(n, 2, int(top), ctx=ctx), TokenLogProbIdsOp(n, ctx=ctx)) if top else r
