@@ -15,7 +15,7 @@ import ctypes
 import torch
 from .. import native_array as _NA
 
-from . import fn, native, stream_ptr, is_bf16, check, supported_float, P, I64, I32
+from . import fn, native, stream_ptr, is_bf16, check, check_device, supported_float, record_native, P, I64, I32
 
 
 def _dc(t, dtype=None):
@@ -104,6 +104,108 @@ def aux_terms(counts, psum, T):
         return coef, l_aux
     coef = counts.float() / float(T)
     return coef, (psum / float(T) * coef).sum() * float(E)
+
+
+# ---- balance loss with counts (moe_balance.hip) --------------------------------------------------
+MAX_EXPERTS = 1024
+_VALID_KINDS = {torch.bool: 0, torch.uint8: 0, torch.int8: 0, torch.float32: 1, torch.bfloat16: 2, torch.int64: 3,
+                torch.int32: 4}
+
+
+class BalanceLoss(object):
+    """Result of ``balance_loss``: ``loss`` fp32 [1], ``counts`` int64 [E], and ``weight`` fp32 [E],
+    d loss / d (sum of the tokens' probabilities of an expert), for the backward pass."""
+    __slots__ = ('loss', 'counts', 'weight')
+
+    def __init__(self, loss, counts, weight):
+        self.loss, self.counts, self.weight = loss, counts, weight
+
+
+def _balance_operands(name, logits, valid):
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or not supported_float(logits):
+        raise ValueError('%s: logits have to be an fp32 or bf16 [tokens, experts] tensor' % name)
+    T, E = logits.shape
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError('%s: 1 to %d experts, got %d' % (name, MAX_EXPERTS, E))
+    x = logits
+    if E > 1 and x.stride(1) != 1 or T > 1 and x.stride(0) < 0:
+        x = _dc(x)
+    if valid is not None:
+        if valid.numel() != T or valid.dtype not in _VALID_KINDS or valid.device != x.device:
+            raise ValueError('%s: valid has to hold one value a token (%d) on %s, got %s %s on %s'
+                             % (name, T, x.device, valid.dtype, tuple(valid.shape), valid.device))
+        valid = _dc(valid).reshape(T)
+    return x, valid, T, E
+
+
+def balance_loss(logits, indices, num_experts, valid=None):
+    """Balance loss of a router and how many choices each expert got.
+
+    With p = softmax(logits) [T, E] (fp32 or bf16; rows may be strided), N the tokens whose
+    ``valid`` [T] is not 0 (None: all), c_e the number of their ``indices`` [T, k] equal to e:
+    loss = E sum_e (c_e / N) (sum_t p[t, e] / N), over the valid tokens.  An index outside [0, E)
+    is a choice not made and is not counted.  Without a valid token the loss is 0."""
+    x, valid, T, E = _balance_operands('balance_loss', logits, valid)
+    if int(num_experts) != E:
+        raise ValueError('balance_loss: %d experts, but logits of %d' % (num_experts, E))
+    if indices.dim() < 1 or indices.shape[0] != T or T and indices.numel() % T or indices.device != x.device:
+        raise ValueError('balance_loss: indices have to be [%d, k] on %s, got %s on %s'
+                         % (T, x.device, tuple(indices.shape), indices.device))
+    idx = indices.reshape(T, -1) if indices.numel() else indices.reshape(T, 0)
+    k = idx.shape[1]
+    if T and k < 1:
+        raise ValueError('balance_loss: at least one choice a token')
+    if idx.dtype != torch.int64:
+        idx = idx.long()
+    if native(x):
+        check_device(x, 'balance_loss')
+        idx = _dc(idx)
+        loss = _NA.empty((1,), dtype=torch.float32, device=x.device)
+        counts = _NA.empty((E,), dtype=torch.int64, device=x.device)
+        weight = _NA.empty((E,), dtype=torch.float32, device=x.device)
+        nws = int(fn('hetu_moe_balance_ws', [I64, I32], I64)(T, E))
+        ws = _NA.empty((nws,), dtype=torch.int32, device=x.device) if nws else None
+        f = fn('hetu_moe_balance_fwd', [P, I64, I64, I32, P, I32, P, I32, P, P, P, P, I32, P])
+        check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, idx.data_ptr(), max(k, 1), ptr_or_none(valid),
+                _VALID_KINDS[valid.dtype] if valid is not None else 0, counts.data_ptr(), weight.data_ptr(),
+                loss.data_ptr(), ptr_or_none(ws), is_bf16(x), stream_ptr()), 'moe_balance')
+        record_native('moe_balance')
+        return BalanceLoss(loss, counts, weight)
+    on = torch.ones(T, dtype=torch.bool, device=x.device) if valid is None else valid != 0
+    chosen = idx[on].reshape(-1)
+    chosen = chosen[(chosen >= 0) & (chosen < E)]
+    counts = torch.bincount(chosen, minlength=E)
+    n = int(on.sum())
+    if n == 0:
+        return BalanceLoss(_NA.zeros(1, device=x.device), counts, _NA.zeros(E, device=x.device))
+    weight = E * counts.double() / (float(n) * n)
+    loss = (weight * torch.softmax(x[on].float(), 1).double().sum(0)).sum().reshape(1)
+    return BalanceLoss(loss.float(), counts, weight.float())
+
+
+def balance_loss_backward(logits, fwd, grad, valid=None):
+    """d logits (contiguous, of the logits' type) from ``grad``, the gradient of the loss (one
+    fp32 value); ``fwd`` is what ``balance_loss`` gave for the same logits and ``valid``.  Tokens
+    that are not valid get 0."""
+    x, valid, T, E = _balance_operands('balance_loss_backward', logits, valid)
+    if fwd.weight.numel() != E or grad.numel() != 1 or grad.device != x.device:
+        raise ValueError('balance_loss_backward: %d experts, weights of %d, a gradient of %s'
+                         % (E, fwd.weight.numel(), tuple(grad.shape)))
+    if native(x):
+        check_device(x, 'balance_loss_backward')
+        grad = _dc(grad, torch.float32)
+        dx = _NA.empty((T, E), dtype=x.dtype, device=x.device)
+        f = fn('hetu_moe_balance_bwd', [P, I64, I64, I32, P, P, P, I32, P, I32, P])
+        check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, fwd.weight.data_ptr(), grad.data_ptr(),
+                ptr_or_none(valid), _VALID_KINDS[valid.dtype] if valid is not None else 0, dx.data_ptr(), is_bf16(x),
+                stream_ptr()), 'moe_balance_bwd')
+        record_native('moe_balance_bwd')
+        return dx
+    p = torch.softmax(x.float(), 1)
+    d = grad.float().reshape(1, 1) * p * (fwd.weight - (p * fwd.weight).sum(1, keepdim=True))
+    if valid is not None:
+        d = torch.where((valid != 0)[:, None], d, torch.zeros_like(d))
+    return d.to(x.dtype)
 
 
 MAX_K = 16   # choices per token the kernels take (moe.hip kMaxK)

@@ -48,7 +48,14 @@ def _fused_locations(topk_indices, k, num_experts):
     return [O.split_op(loc, axes=[1], indices=[i], splits=[k]) for i in range(k)]
 
 
-def topkgating(logits, k, capacity_factor, num_tokens, num_experts, embed_dim=None, fused=True):
+def topkgating(logits, k, capacity_factor, num_tokens, num_experts, embed_dim=None, fused=True, token_mask=None):
+    """``token_mask`` [tokens], 0 for padding: the balance loss then counts the other tokens alone
+    (``balance_loss_op``); routing and capacity are the same with and without it."""
+    if token_mask is not None:
+        _, indices_s, location_s, gates_s, capacity = topkgating(logits, k, capacity_factor, num_tokens, num_experts,
+                                                                 embed_dim, fused)
+        l_aux, _ = O.balance_loss_op(logits, indices_s, num_experts, token_mask)
+        return l_aux, indices_s, location_s, gates_s, capacity
     capacity = k * math.ceil((num_tokens / num_experts) * capacity_factor)
     if fused and k <= 8 and num_experts <= 512:
         from ..ops.moe import topk_gating_op
@@ -92,9 +99,9 @@ class TopKGate(_GateBase):
                          initializer, name)
         self.fused = fused
 
-    def __call__(self, x):
+    def __call__(self, x, token_mask=None):
         return topkgating(self._logits(x), self.top_k, self.capacity_factor, self.num_tokens,
-                          self.num_experts, fused=self.fused)
+                          self.num_experts, fused=self.fused, token_mask=token_mask)
 
 
 class KTop1Gate(_GateBase):
@@ -330,11 +337,15 @@ class MoELayer(BaseLayer):
         self.all2all_size = all2all_size or 1
         self.device_id, self.top = device_id or 0, top
 
-    def __call__(self, x):
+    def __call__(self, x, token_mask=None):
+        """``token_mask`` [tokens] (TopKGate): 0 for padding tokens, left out of the balance loss"""
         reshaped = O.array_reshape_op(x, [-1, self.embed_dim])
+        if token_mask is not None and not isinstance(self.gate, TopKGate):
+            raise ValueError('%s takes no token mask' % type(self.gate).__name__)
         if self.name == 'BalanceAssignmentLayer' or isinstance(self.gate, BalanceAssignmentGate):
             return self._base_layer(reshaped)
-        l_aux, indices_s, location_s, gates_s, capacity = self.gate(reshaped)
+        l_aux, indices_s, location_s, gates_s, capacity = \
+            self.gate(reshaped) if token_mask is None else self.gate(reshaped, token_mask)
         return _dispatch_and_run(self, reshaped, indices_s, location_s, gates_s, capacity), l_aux
 
     def _base_layer(self, reshaped):

@@ -50,7 +50,7 @@ from .moe import (layout_transform_op, layout_transform_gradient_op, reverse_lay
                   reverse_layout_transform_gradient_gate_op, reverse_layout_transform_no_gate_op,
                   reverse_layout_transform_no_gate_gradient_op, balance_assignment_op,
                   sam_group_sum_op, sam_max_op, sammax_grad_op, group_topk_idx_op, topk_gating_op,
-                  topk_locations_op)
+                  topk_locations_op, balance_loss_op)
 from .ps_ops import (parameterServerCommunicate_op, parameterServerSparsePull_op,
                      ParameterServerCommunicateOp, ParameterServerSparsePullOp)
 from .executor import Executor, HetuConfig, gradients, find_topo_sort

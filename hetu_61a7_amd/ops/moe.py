@@ -537,3 +537,70 @@ class TopKLocationsOp(Op):
 
 def topk_locations_op(indices, num_experts, ctx=None):
     return TopKLocationsOp(indices, num_experts, ctx=ctx)
+
+
+# ---------------------------------------------------------------------------
+# Balance loss from a router's logits over the valid tokens, with the experts' counts.
+class BalanceLossOp(Op):
+    def __init__(self, logits, indices_s, num_experts, valid=None, ctx=None):
+        indices_s = list(indices_s) if isinstance(indices_s, (list, tuple)) else [indices_s]
+        super().__init__(BalanceLossOp, [logits] + indices_s + ([valid] if valid is not None else []), ctx)
+        self.k, self.num_experts, self.has_valid = len(indices_s), int(num_experts), valid is not None
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        from .nn import AuxResult
+        r = KM.balance_loss(input_vals[0], _stack(input_vals[1:1 + self.k]), self.num_experts,
+                            input_vals[-1] if self.has_valid else None)
+        return AuxResult(r.loss, r)
+
+    def gradient(self, output_grad):
+        g = BalanceLossGradientOp(output_grad, self, ctx=self.raw_ctx)
+        return [g] + [None] * (len(self.inputs) - 1)
+
+    def infer_shape(self, input_shapes):
+        return (1,)
+
+
+class BalanceLossGradientOp(Op):
+    aux_inputs = (2,)
+
+    def __init__(self, grad, fwd, ctx=None):
+        super().__init__(BalanceLossGradientOp, [fwd.inputs[0], grad, fwd] + (fwd.inputs[-1:] if fwd.has_valid else []), ctx)
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        x, g, r = input_vals[:3]
+        if g.numel() > 1 and all(s == 0 for s in g.stride()):
+            g = g.as_strided((1,), (1,))
+        return KM.balance_loss_backward(x, r, g, input_vals[3] if len(input_vals) > 3 else None)
+
+    def gradient(self, output_grad):
+        raise NotImplementedError
+
+    def infer_shape(self, input_shapes):
+        return input_shapes[0]
+
+
+class BalanceCountsOp(Op):
+    aux_inputs = (0,)
+
+    def __init__(self, node, ctx=None):
+        super().__init__(BalanceCountsOp, [node], ctx)
+        self.num_experts = node.num_experts
+
+    def compute(self, input_vals, output_val=None, stream_handle=None):
+        return input_vals[0].counts
+
+    def gradient(self, output_grad):
+        return [None]
+
+    def infer_shape(self, input_shapes):
+        return (self.num_experts,)
+
+
+def balance_loss_op(logits, indices_s, num_experts, valid=None, ctx=None):
+    """(loss [1], counts [num_experts]) of a router: the balance loss
+    E sum_e (c_e / N) (P_e / N) of ``logits`` [T, E] and the chosen experts ``indices_s`` ([T, k], or
+    one [T] node a choice) over the N tokens whose ``valid`` [T] is not 0, and the counts c_e
+    (int64).  The loss is differentiable with respect to the logits (``kernels.moe``)."""
+    n = BalanceLossOp(logits, indices_s, num_experts, valid, ctx=ctx)
+    return n, BalanceCountsOp(n, ctx=ctx)
