@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import torch
 
-from . import fn, native, stream_ptr, check, check_device, ptr, P, I64, I32, F32
+from . import fn, native, stream_ptr, check, check_device, ptr, record_native, P, I64, I32, F32
 
 MODES = dict(sgd=0, momentum=1, nesterov=2, adagrad=3, adam=4, adamw=5, lamb=6)
 
@@ -174,6 +174,7 @@ def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.
         check(f(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale.data_ptr(), v_scale.data_ptr(),
                 ptr(shadow), n, lr, beta1, beta2, 1.0 - beta1, 1.0 - beta2, 1.0 - beta1t, 1.0 - beta2t, eps,
                 wd, gscale, ptr(dyn), _i64(seed), stream_ptr()), 'adamw8')
+        record_native('adamw8')
         return
     if dyn is not None:
         lr, _, _, gscale, step, c1, c2 = [float(x) for x in dyn.tolist()]
