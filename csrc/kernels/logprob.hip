@@ -22,9 +22,7 @@
 namespace hetu {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr int kLpThreads = 256;      // a block a row
 constexpr int kMaxTop = 64;
-constexpr int kCand = 1024;          // candidate keys kept in LDS; more take the slow way
 
 struct Lse { float m, s, u; };       // running maximum, sum, base-2 weighted sum
 
@@ -33,12 +31,15 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f
 // base-2 exponent's floor in products e * t: e is 0 there, and t may be -inf
 constexpr float kFloor2 = -200.f;
 
+// v_exp_f32: results below 2^-126 are 0, which sums of at least 1 do not feel
+__device__ __forceinline__ float exp2_(float t) { return __builtin_amdgcn_exp2f(t); }
+
 __device__ __forceinline__ Lse lse_join(const Lse& a, const Lse& b) {
   Lse r;
   r.m = fmaxf(a.m, b.m);
   const float sh = shift_of(r.m);
   const float da = (a.m - sh) * kLog2e, db = (b.m - sh) * kLog2e;
-  const float ea = exp2f(da), eb = exp2f(db);
+  const float ea = exp2_(da), eb = exp2_(db);
   r.s = a.s * ea + b.s * eb;
   r.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + eb * (b.u + fmaxf(db, kFloor2) * b.s);
   return r;
@@ -85,15 +86,18 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)~(unsigned)key; }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprob_k(const T* __restrict__ logits, int64_t stride,
-                                                              const int64_t* __restrict__ ids, int V, int n,
-                                                              int64_t ignored, float* __restrict__ out,
-                                                              float* __restrict__ stats, int64_t* __restrict__ top) {
-  constexpr int NT = kLpThreads, VE = Vec<T>::N;
+// One block of NT threads a row.
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
+                                                      const int64_t* __restrict__ ids, int V, int n, int64_t ignored,
+                                                      float* __restrict__ out, float* __restrict__ stats,
+                                                      int64_t* __restrict__ top) {
+  constexpr int VE = Vec<T>::N, U = 4;              // granules under way at once
+  constexpr int NG = TOP ? (NT < 256 ? NT : 256) : 1, PER = TOP ? NT / NG : 1;   // groups of threads that give a sample
+  constexpr int CAND = NT < 256 ? 512 : 1024;       // candidates kept in LDS; more take the slow way
   __shared__ Lse part[NT / 64];
-  __shared__ uint64_t keys[NT], cand[kCand], bound;
-  __shared__ int flagged[NT], n_flagged, n_cand;
+  __shared__ uint64_t keys[NG], cand[TOP ? CAND : 1], bound;
+  __shared__ int flagged[NG], n_flagged, n_cand;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int64_t t = ids[row];
@@ -107,29 +111,44 @@ __global__ void __launch_bounds__(kLpThreads) token_logprob_k(const T* __restric
   const Row<T> r(logits + row * stride, V);
   Lse a = {-INFINITY, 0.f, 0.f};
   int best = tid;
-  for (int j = tid; j < r.ng; j += NT) {
-    float v[VE];
-    r.load(j, v);
-    float vm = v[0];
+  for (int j = tid; j < r.ng; j += U * NT) {
+    float v[U][VE];
 #pragma unroll
-    for (int k = 1; k < VE; ++k) vm = fmaxf(vm, v[k]);
-    if (vm > a.m) best = j;
-    Lse b = {fmaxf(a.m, vm), 0.f, 0.f};
-    const float sh = shift_of(b.m);
+    for (int u = 0; u < U; ++u) {
+      if (j + u * NT < r.ng) {
+        r.load(j + u * NT, v[u]);
+      } else {
 #pragma unroll
-    for (int k = 0; k < VE; ++k) {
-      const float d = (v[k] - sh) * kLog2e, e = exp2f(d);
-      b.s += e;
-      b.u += e * fmaxf(d, kFloor2);
+        for (int k = 0; k < VE; ++k) v[u][k] = -INFINITY;
+      }
     }
-    const float da = (a.m - sh) * kLog2e, ea = exp2f(da);
-    a.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + b.u;
-    a.s = a.s * ea + b.s;
-    a.m = b.m;
+    float m = a.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float vm = v[u][0];
+#pragma unroll
+      for (int k = 1; k < VE; ++k) vm = fmaxf(vm, v[u][k]);
+      if (TOP && vm > m) best = j + u * NT;
+      m = fmaxf(m, vm);
+    }
+    const float sh = shift_of(m);
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        const float d = (v[u][k] - sh) * kLog2e, e = exp2_(d);
+        s += e;
+        w += e * fmaxf(d, kFloor2);
+      }
+    const float da = (a.m - sh) * kLog2e, ea = exp2_(da);
+    a.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + w;
+    a.s = a.s * ea + s;
+    a.m = m;
   }
   // this thread's largest element, for the selection below
   uint64_t mine = 0;
-  if (n > 0 && tid < r.ng) {
+  if (TOP && tid < r.ng) {
     float v[VE];
     r.load(best, v);
     const int e0 = best * VE - r.off;
@@ -144,13 +163,22 @@ __global__ void __launch_bounds__(kLpThreads) token_logprob_k(const T* __restric
     const Lse b = {__shfl_xor(a.m, s, 64), __shfl_xor(a.s, s, 64), __shfl_xor(a.u, s, 64)};
     a = lse_join(a, b);
   }
-  if ((tid & 63) == 0) part[tid >> 6] = a;
-  if (n > 0) keys[tid] = mine;
-  if (tid == 0) { bound = 0; n_flagged = 0; n_cand = 0; }
-  __syncthreads();
-  a = part[0];
+  if (NT > 64 && (tid & 63) == 0) part[tid >> 6] = a;
+  if (TOP) {
 #pragma unroll
-  for (int w = 1; w < NT / 64; ++w) a = lse_join(a, part[w]);
+    for (int s = 1; s < PER; s <<= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)mine, s, 64);
+      if (other > mine) mine = other;
+    }
+    if (tid % PER == 0) keys[tid / PER] = mine;
+    if (tid == 0) { n_flagged = 0; n_cand = 0; }
+  }
+  __syncthreads();
+  if (NT > 64) {
+    a = part[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) a = lse_join(a, part[w]);
+  }
   const bool empty = a.m == -INFINITY && a.s == 0.f;
   const float log2s = log2f(a.s), logs = log2s * kLn2;
   if (tid == 0) {
@@ -160,49 +188,63 @@ __global__ void __launch_bounds__(kLpThreads) token_logprob_k(const T* __restric
     stats[row * 2] = a.m;
     stats[row * 2 + 1] = log2s;
   }
-  if (n == 0) return;
-  int rank = 0;
-  for (int i = 0; i < NT; ++i) rank += keys[i] > mine;
-  if (mine != 0 && rank == n - 1) bound = mine;
-  __syncthreads();
-  const uint64_t least = bound;          // 0 where fewer than n threads have an element: all are candidates
-  if (mine != 0 && mine >= least) flagged[atomicAdd(&n_flagged, 1)] = tid;
-  __syncthreads();
-  const int J = (r.ng + NT - 1) / NT, todo = n_flagged * J;
-  for (int i = tid; i < todo; i += NT) {
-    const int j = (i % J) * NT + flagged[i / J];
-    if (j >= r.ng) continue;
-    float v[VE];
-    r.load(j, v);
-    const int e0 = j * VE - r.off;
+  if constexpr (TOP) {
+    // the n-th largest sample, bit by bit from the highest: the largest key that n samples reach (0
+    // where fewer than n threads have an element: then all are candidates)
+    if (tid < 64) {
+      constexpr int Q = NG / 64;
+      uint64_t k[Q], b = 0;
 #pragma unroll
-    for (int k = 0; k < VE; ++k) {
-      const uint64_t key = key_of(v[k], e0 + k);
-      if (e0 + k >= 0 && e0 + k < V && key >= least) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at < kCand) cand[at] = key;
+      for (int q = 0; q < Q; ++q) k[q] = keys[tid + q * 64];
+      for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t c = b | (1ull << bit);
+        int reach = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(k[q] >= c));
+        if (reach >= n) b = c;
+        if (reach == n) break;           // these n are the ones: any bound between them and the next will do
+      }
+      if (tid == 0) bound = b;
+    }
+    __syncthreads();
+    const uint64_t least = bound;
+    if (tid < NG && keys[tid] != 0 && keys[tid] >= least) flagged[atomicAdd(&n_flagged, 1)] = tid;
+    __syncthreads();
+    const int J = (r.ng + NT - 1) / NT * PER, todo = n_flagged * J;
+    for (int i = tid; i < todo; i += NT) {
+      const int f = flagged[i / J], jj = i % J;
+      const int j = (jj / PER) * NT + f * PER + jj % PER;
+      if (j >= r.ng) continue;
+      float v[VE];
+      r.load(j, v);
+      const int e0 = j * VE - r.off;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        const uint64_t key = key_of(v[k], e0 + k);
+        if (e0 + k >= 0 && e0 + k < V && key >= least) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < CAND) cand[at] = key;
+        }
       }
     }
-  }
-  __syncthreads();
-  const int C = n_cand;
-  if (C <= kCand) {
-    for (int c = tid; c < C; c += NT) {
-      const uint64_t key = cand[c];
-      int at = 0;
-      for (int i = 0; i < C; ++i) at += cand[i] > key;
-      if (at < n) {
-        o[2 + at] = empty ? -INFINITY : (key_value(key) - a.m) - logs;
-        top[row * n + at] = key_index(key);
+    __syncthreads();
+    const int C = n_cand;
+    if (C <= CAND) {
+      for (int c = tid; c < C; c += NT) {
+        const uint64_t key = cand[c];
+        int at = 0;
+        for (int i = 0; i < C; ++i) at += cand[i] > key;
+        if (at < n) {
+          o[2 + at] = empty ? -INFINITY : (key_value(key) - a.m) - logs;
+          top[row * n + at] = key_index(key);
+        }
       }
+      return;
     }
-    return;
-  }
-  // many elements of few threads above the bound: n rounds of the largest below the last one
-  uint64_t last = ~0ull;
-  for (int i = 0; i < n; ++i) {
-    uint64_t most = 0;
-    if (mine != 0 && mine >= least) {
+    // many elements of few threads above the bound: n rounds of the largest below the last one
+    uint64_t last = ~0ull;
+    for (int i = 0; i < n; ++i) {
+      uint64_t most = 0;
       for (int j = tid; j < r.ng; j += NT) {
         float v[VE];
         r.load(j, v);
@@ -213,78 +255,95 @@ __global__ void __launch_bounds__(kLpThreads) token_logprob_k(const T* __restric
           if (e0 + k >= 0 && e0 + k < V && key < last && key > most) most = key;
         }
       }
-    }
-    __syncthreads();
-    keys[tid] = most;
-    __syncthreads();
-    most = 0;
-    for (int k = 0; k < NT; ++k) most = keys[k] > most ? keys[k] : most;
-    last = most;
-    if (tid == 0) {
-      o[2 + i] = empty ? -INFINITY : (key_value(most) - a.m) - logs;
-      top[row * n + i] = key_index(most);
+#pragma unroll
+      for (int s = 32; s > 0; s >>= 1) {
+        const uint64_t other = __shfl_xor((unsigned long long)most, s, 64);
+        if (other > most) most = other;
+      }
+      __syncthreads();
+      if ((tid & 63) == 0) keys[tid >> 6] = most;
+      __syncthreads();
+      for (int w = 0; w < NT / 64; ++w) most = keys[w] > most ? keys[w] : most;
+      last = most;
+      if (tid == 0) {
+        o[2 + i] = empty ? -INFINITY : (key_value(most) - a.m) - logs;
+        top[row * n + i] = key_index(most);
+      }
     }
   }
 }
 
+// A block takes kBwdGranules granules of a row, the last row first: the logits that the forward
+// pass read last are still in the last-level cache.
+constexpr int kBwdThreads = 256, kBwdU = 4, kBwdGranules = kBwdThreads * kBwdU * 2;
+
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprob_bwd_k(const T* __restrict__ logits, int64_t stride,
-                                                                  const int64_t* __restrict__ ids, int V, int n,
-                                                                  int64_t ignored, const float* __restrict__ out,
-                                                                  const float* __restrict__ stats,
-                                                                  const int64_t* __restrict__ top,
-                                                                  const float* __restrict__ grad, T* __restrict__ dx) {
-  constexpr int NT = kLpThreads, VE = Vec<T>::N;
+__global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __restrict__ logits, int64_t stride,
+                                                                   const int64_t* __restrict__ ids, int V, int n,
+                                                                   int64_t ignored, int chunks,
+                                                                   const float* __restrict__ out,
+                                                                   const float* __restrict__ stats,
+                                                                   const int64_t* __restrict__ top,
+                                                                   const float* __restrict__ grad, T* __restrict__ dx) {
+  constexpr int NT = kBwdThreads, VE = Vec<T>::N, U = kBwdU;
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const unsigned at = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = at / chunks;
+  const int chunk = at % chunks;
   const int64_t t = ids[row];
   T* d = dx + row * (int64_t)V;
   const float m = stats[row * 2], log2s = stats[row * 2 + 1];
   const bool dead = t < 0 || t >= V || t == ignored || (m == -INFINITY && log2s == -INFINITY);
   const Row<T> r(logits + row * stride, V), w(d, V);
   const float* g = grad + row * (2 + n);
-  float all = 0.f, gh = 0.f, h = 0.f;
+  float all = 0.f, gh = 0.f;
   if (!dead) {
     all = g[0];
     for (int i = 0; i < n; ++i) all += g[2 + i];
     gh = g[1] * kLn2;
-    h = out[row * (2 + n) + 1];
-    all += g[1] * h;
+    all += g[1] * out[row * (2 + n) + 1];
   }
   const float sh = shift_of(m);
   const auto slope = [&](float x) {
     const float l = (x - sh) * kLog2e - log2s;
-    return -exp2f(l) * (all + gh * fmaxf(l, kFloor2));
+    return -exp2_(l) * (all + gh * fmaxf(l, kFloor2));
   };
-  if (r.off == w.off) {
-    for (int j = tid; j < w.ng; j += NT) {
-      float v[VE];
-      if (!dead) {
-        r.load(j, v);
+  const int j0 = chunk * kBwdGranules, j1 = j0 + kBwdGranules < w.ng ? j0 + kBwdGranules : w.ng;
+  if (dead || r.off == w.off) {
+    for (int j = j0 + tid; j < j1; j += U * NT) {
+      float v[U][VE];
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[k] = slope(v[k]);
-      } else {
+      for (int u = 0; u < U; ++u)
+        if (!dead && j + u * NT < j1) r.load(j + u * NT, v[u]);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[k] = 0.f;
-      }
-      const int64_t e0 = (int64_t)j * VE - w.off;
-      if (w.full(j)) {
-        store_vec<T>(d + e0, v);
-      } else {
+      for (int u = 0; u < U; ++u) {
+        const int ju = j + u * NT;
+        if (ju >= j1) break;
 #pragma unroll
-        for (int k = 0; k < VE; ++k)
-          if (e0 + k >= 0 && e0 + k < V) d[e0 + k] = from_f<T>(v[k]);
+        for (int k = 0; k < VE; ++k) v[u][k] = dead ? 0.f : slope(v[u][k]);
+        const int64_t e0 = (int64_t)ju * VE - w.off;
+        if (w.full(ju)) {
+          store_vec<T>(d + e0, v[u]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VE; ++k)
+            if (e0 + k >= 0 && e0 + k < V) d[e0 + k] = from_f<T>(v[u][k]);
+        }
       }
     }
-  } else {
-    for (int e = tid; e < V; e += NT) d[e] = from_f<T>(dead ? 0.f : slope(to_f(r.x[e])));
+  } else {         // rows of another alignment than the gradient's
+    const int e0 = j0 * VE - w.off, e1 = j1 * VE - w.off;
+    for (int e = (e0 < 0 ? 0 : e0) + tid; e < (e1 < V ? e1 : V); e += NT) d[e] = from_f<T>(slope(to_f(r.x[e])));
   }
   if (dead) return;
-  // the given token and the alternatives once more, each with its own terms: rounded once
+  // this chunk's part of the given token and the alternatives once more, each with its own terms:
+  // rounded once
   __syncthreads();
   for (int i = tid; i <= n; i += NT) {
     const int64_t e = i == 0 ? t : top[row * n + i - 1];
     if (e < 0 || e >= V) continue;
+    const int j = (int)((e + w.off) / VE);
+    if (j < j0 || j >= j1) continue;
     float s = slope(to_f(r.x[e]));
     if (e == t) s += g[0];
     for (int k = 0; k < n; ++k)
@@ -297,16 +356,25 @@ __global__ void __launch_bounds__(kLpThreads) token_logprob_bwd_k(const T* __res
 
 using namespace hetu;
 
+template <typename T>
+static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n, int64_t ignored,
+                       float* out, float* stats, int64_t* top, hipStream_t st) {
+#define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), dim3((unsigned)R), dim3(NT), 0, st, \
+                                       (const T*)logits, stride, ids, V, n, ignored, out, stats, top)
+  const int64_t bytes = (int64_t)V * sizeof(T);
+  if (bytes <= 4096) { if (n) GO(64, true); else GO(64, false); }
+  else if (bytes >= 32768 && R <= 512) { if (n) GO(1024, true); else GO(1024, false); }
+  else { if (n) GO(256, true); else GO(256, false); }
+#undef GO
+}
+
 HETU_API int hetu_token_logprob(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n,
                                 int64_t ignored, float* out, float* stats, int64_t* top, int is_bf16,
                                 hipStream_t st) {
   if (R <= 0) return 0;
   if (V < 1 || n < 0 || n > kMaxTop || n > V || R > 0x7fffffff) return (int)hipErrorInvalidValue;
-  const dim3 grid((unsigned)R), block(kLpThreads);
-  if (is_bf16)
-    hipLaunchKernelGGL(token_logprob_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, out, stats, top);
-  else
-    hipLaunchKernelGGL(token_logprob_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, out, stats, top);
+  if (is_bf16) launch_fwd<bf16>(logits, stride, ids, R, V, n, ignored, out, stats, top, st);
+  else launch_fwd<float>(logits, stride, ids, R, V, n, ignored, out, stats, top, st);
   HETU_LAUNCH_CHECK();
   return 0;
 }
@@ -315,12 +383,14 @@ HETU_API int hetu_token_logprob_bwd(const void* logits, int64_t stride, const in
                                     int64_t ignored, const float* out, const float* stats, const int64_t* top,
                                     const float* grad, void* dx, int is_bf16, hipStream_t st) {
   if (R <= 0) return 0;
-  if (V < 1 || n < 0 || n > kMaxTop || n > V || R > 0x7fffffff) return (int)hipErrorInvalidValue;
-  const dim3 grid((unsigned)R), block(kLpThreads);
+  const int VE = is_bf16 ? 8 : 4;
+  const int64_t chunks = ((int64_t)V + 2 * VE - 2 + (int64_t)VE * kBwdGranules - 1) / ((int64_t)VE * kBwdGranules);
+  if (V < 1 || n < 0 || n > kMaxTop || n > V || R * chunks > 0x7fffffff) return (int)hipErrorInvalidValue;
+  const dim3 grid((unsigned)(R * chunks)), block(kBwdThreads);
   if (is_bf16)
-    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, out, stats, top, grad, (bf16*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, (int)chunks, out, stats, top, grad, (bf16*)dx);
   else
-    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, out, stats, top, grad, (float*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, (int)chunks, out, stats, top, grad, (float*)dx);
   HETU_LAUNCH_CHECK();
   return 0;
 }
