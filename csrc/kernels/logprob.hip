@@ -45,6 +45,20 @@ __device__ __forceinline__ Lse lse_join(const Lse& a, const Lse& b) {
   return r;
 }
 
+typedef unsigned Raw __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void unpack(const Raw& q, float (&v)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(q[k]);
+}
+__device__ __forceinline__ void unpack(const Raw& q, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = __uint_as_float(q[k] << 16);
+    v[2 * k + 1] = __uint_as_float(q[k] & 0xffff0000u);
+  }
+}
+
 // A row of V elements as 16-byte granules from the aligned address at or below its start:
 // granule j holds elements j * VE - off + (0 .. VE - 1), of which the first and the last granule
 // may lack some.
@@ -52,14 +66,18 @@ template <typename T>
 struct Row {
   static constexpr int VE = Vec<T>::N;
   const T* x;
-  int V, off, ng;
+  int V, off, ng, f0, f1;      // granules 0 .. ng - 1; those of f0 .. f1 - 1 are whole
   __device__ __forceinline__ Row(const T* x_, int V_) : x(x_), V(V_) {
     off = (int)(((uintptr_t)x & 15) / sizeof(T));
     ng = (int)(((int64_t)off + V + VE - 1) / VE);
+    f0 = off ? 1 : 0;
+    f1 = (int)(((int64_t)off + V) / VE);
   }
-  __device__ __forceinline__ bool full(int j) const {
-    const int64_t e0 = (int64_t)j * VE - off;
-    return e0 >= 0 && e0 + VE <= V;
+  __device__ __forceinline__ bool has_head() const { return f0 > 0; }
+  __device__ __forceinline__ bool has_tail() const { return f1 < ng && ng - 1 >= f0; }
+  // a whole granule as it is in memory
+  __device__ __forceinline__ Raw raw(int j) const {
+    return *reinterpret_cast<const Raw*>(x - off + (int64_t)j * VE);
   }
   // elements of granule j, -inf where the row has none
   __device__ __forceinline__ void load(int j, float (&v)[VE]) const {
@@ -86,7 +104,37 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)~(unsigned)key; }
 
-// One block of NT threads a row.
+// takes U granules v (numbers j, j + step, ..) into the running sums; `best`: the granule with the
+// first of the largest values so far
+template <int U, int VE, bool TOP>
+__device__ __forceinline__ void lse_take(Lse& a, int& best, const float (&v)[U][VE], int j, int step) {
+  float m = a.m;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float vm = v[u][0];
+#pragma unroll
+    for (int k = 1; k < VE; ++k) vm = fmaxf(vm, v[u][k]);
+    if (TOP && (vm > m || best < 0)) best = j + u * step;
+    m = fmaxf(m, vm);
+  }
+  const float sh = shift_of(m);
+  float s = 0.f, w = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+      const float d = (v[u][k] - sh) * kLog2e, e = exp2_(d);
+      s += e;
+      w += e * fmaxf(d, kFloor2);
+    }
+  const float da = (a.m - sh) * kLog2e, ea = exp2_(da);
+  a.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + w;
+  a.s = a.s * ea + s;
+  a.m = m;
+}
+
+// One block of NT threads a row: thread i takes the whole granules f0 + i, f0 + i + NT, .., U of
+// them under way at once; thread 0 the head and the last thread the tail that are not whole.
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
                                                       const int64_t* __restrict__ ids, int V, int n, int64_t ignored,
@@ -110,45 +158,36 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
   }
   const Row<T> r(logits + row * stride, V);
   Lse a = {-INFINITY, 0.f, 0.f};
-  int best = tid;
-  for (int j = tid; j < r.ng; j += U * NT) {
+  int best = -1;
+  int j = r.f0 + tid;
+  for (; j + (U - 1) * NT < r.f1; j += U * NT) {
+    Raw q[U];
     float v[U][VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (j + u * NT < r.ng) {
-        r.load(j + u * NT, v[u]);
-      } else {
+    for (int u = 0; u < U; ++u) q[u] = r.raw(j + u * NT);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[u][k] = -INFINITY;
-      }
+    for (int u = 0; u < U; ++u) unpack(q[u], v[u]);
+    lse_take<U, VE, TOP>(a, best, v, j, NT);
+  }
+  for (; j < r.f1; j += NT) {
+    float v[1][VE];
+    unpack(r.raw(j), v[0]);
+    lse_take<1, VE, TOP>(a, best, v, j, NT);
+  }
+  if ((tid == 0 && r.has_head()) || (tid == NT - 1 && r.has_tail())) {
+    float v[1][VE];
+    if (tid == 0 && r.has_head()) {
+      r.load(0, v[0]);
+      lse_take<1, VE, TOP>(a, best, v, 0, NT);
     }
-    float m = a.m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float vm = v[u][0];
-#pragma unroll
-      for (int k = 1; k < VE; ++k) vm = fmaxf(vm, v[u][k]);
-      if (TOP && vm > m) best = j + u * NT;
-      m = fmaxf(m, vm);
+    if (tid == NT - 1 && r.has_tail()) {
+      r.load(r.ng - 1, v[0]);
+      lse_take<1, VE, TOP>(a, best, v, r.ng - 1, NT);
     }
-    const float sh = shift_of(m);
-    float s = 0.f, w = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int k = 0; k < VE; ++k) {
-        const float d = (v[u][k] - sh) * kLog2e, e = exp2_(d);
-        s += e;
-        w += e * fmaxf(d, kFloor2);
-      }
-    const float da = (a.m - sh) * kLog2e, ea = exp2_(da);
-    a.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + w;
-    a.s = a.s * ea + s;
-    a.m = m;
   }
   // this thread's largest element, for the selection below
   uint64_t mine = 0;
-  if (TOP && tid < r.ng) {
+  if (TOP && best >= 0) {
     float v[VE];
     r.load(best, v);
     const int e0 = best * VE - r.off;
@@ -210,11 +249,18 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     const uint64_t least = bound;
     if (tid < NG && keys[tid] != 0 && keys[tid] >= least) flagged[atomicAdd(&n_flagged, 1)] = tid;
     __syncthreads();
-    const int J = (r.ng + NT - 1) / NT * PER, todo = n_flagged * J;
+    // granules of a flagged group: its threads' whole ones, then the head or tail that is theirs
+    const int J = r.f1 > r.f0 ? (r.f1 - r.f0 + NT - 1) / NT * PER : 0, todo = n_flagged * (J + 1);
     for (int i = tid; i < todo; i += NT) {
-      const int f = flagged[i / J], jj = i % J;
-      const int j = (jj / PER) * NT + f * PER + jj % PER;
-      if (j >= r.ng) continue;
+      const int f = flagged[i / (J + 1)], jj = i % (J + 1);
+      int j = r.f0 + (jj / PER) * NT + f * PER + jj % PER;
+      if (jj == J) {
+        if (f == 0 && r.has_head()) j = 0;
+        else if (f == NG - 1 && r.has_tail()) j = r.ng - 1;
+        else continue;
+      } else if (j >= r.f1) {
+        continue;
+      }
       float v[VE];
       r.load(j, v);
       const int e0 = j * VE - r.off;
@@ -309,28 +355,46 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
     return -exp2_(l) * (all + gh * fmaxf(l, kFloor2));
   };
   const int j0 = chunk * kBwdGranules, j1 = j0 + kBwdGranules < w.ng ? j0 + kBwdGranules : w.ng;
-  if (dead || r.off == w.off) {
-    for (int j = j0 + tid; j < j1; j += U * NT) {
-      float v[U][VE];
+  const auto take = [&](int j) {       // one granule, whole or not
+    float v[VE];
+    const int64_t e0 = (int64_t)j * VE - w.off;
+    if (dead) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (!dead && j + u * NT < j1) r.load(j + u * NT, v[u]);
+      for (int k = 0; k < VE; ++k) v[k] = 0.f;
+    } else {
+      r.load(j, v);
+#pragma unroll
+      for (int k = 0; k < VE; ++k) v[k] = slope(v[k]);
+    }
+    if (j >= w.f0 && j < w.f1) {
+      store_vec<T>(d + e0, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VE; ++k)
+        if (e0 + k >= 0 && e0 + k < V) d[e0 + k] = from_f<T>(v[k]);
+    }
+  };
+  if (dead) {
+    for (int j = j0 + tid; j < j1; j += NT) take(j);
+  } else if (r.off == w.off) {
+    const int a0 = j0 < w.f0 ? w.f0 : j0, a1 = j1 < w.f1 ? j1 : w.f1;
+    int j = a0 + tid;
+    for (; j + (U - 1) * NT < a1; j += U * NT) {
+      Raw q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = r.raw(j + u * NT);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int ju = j + u * NT;
-        if (ju >= j1) break;
+        float v[VE];
+        unpack(q[u], v);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[u][k] = dead ? 0.f : slope(v[u][k]);
-        const int64_t e0 = (int64_t)ju * VE - w.off;
-        if (w.full(ju)) {
-          store_vec<T>(d + e0, v[u]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < VE; ++k)
-            if (e0 + k >= 0 && e0 + k < V) d[e0 + k] = from_f<T>(v[u][k]);
-        }
+        for (int k = 0; k < VE; ++k) v[k] = slope(v[k]);
+        store_vec<T>(d + (int64_t)(j + u * NT) * VE - w.off, v);
       }
     }
+    for (; j < a1; j += NT) take(j);
+    if (tid == 0 && chunk == 0 && w.has_head()) take(0);
+    if (tid == NT - 1 && chunk == chunks - 1 && w.has_tail()) take(w.ng - 1);
   } else {         // rows of another alignment than the gradient's
     const int e0 = j0 * VE - w.off, e1 = j1 * VE - w.off;
     for (int e = (e0 < 0 ? 0 : e0) + tid; e < (e1 < V ? e1 : V); e += NT) d[e] = from_f<T>(slope(to_f(r.x[e])));

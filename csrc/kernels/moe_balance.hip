@@ -93,25 +93,31 @@ __global__ void __launch_bounds__(kBlThreads) balance_part_k(const T* __restrict
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  // the choices, one a thread: (token, choice) advances by 256 choices without a division
+  {
+    const int dt = kBlThreads / k, dc = kBlThreads - dt * k;
+    int64_t t = t0 + tid / k;
+    int c = tid % k;
+    while (t < t1) {
+      if (token_on(valid, kind, t)) {
+        const int64_t e = idx[t * k + c];
+        if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
+      }
+      t += dt;
+      c += dc;
+      if (c >= k) { c -= k; ++t; }
+    }
+  }
   int count = 0;
   for (int64_t t = t0 + group; t < t1; t += (int64_t)groups * U) {
     float p[U][N];
     bool on[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u) {      // a token that is not valid: the row of t0 in its place, unused
       const int64_t tu = t + (int64_t)u * groups;
       on[u] = tu < t1 && token_on(valid, kind, tu);
-      if (on[u]) {
-        row_load<T, V, NJ>(x + tu * stride, E, G, lane, p[u]);
-        for (int c = lane; c < k; c += G) {
-          const int64_t e = idx[tu * k + c];
-          if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
-        }
-        ++count;
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[u][i] = 0.f;
-      }
+      row_load<T, V, NJ>(x + (on[u] ? tu : t0) * stride, E, G, lane, p[u]);
+      count += on[u];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(kBlThreads) balance_part_k(const T* __restrict
 // Counts, the weights of the backward pass and the loss from the blocks' sums: EB experts a
 // block, the partial sums of one expert over 1024 / EB threads, all in a fixed order.  The block
 // that comes last adds up the blocks' parts of the loss, in order too.
-constexpr int kJoinThreads = 1024, kJoinExperts = 32;
+constexpr int kJoinThreads = 1024, kJoinExperts = 16;
 
 __global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __restrict__ psum,
                                                                const int* __restrict__ pcnt, int blocks, int E, int EB,
@@ -193,9 +199,14 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __re
     sums[tid] = l;
   }
   __syncthreads();
+  if (tid < 64) {
+    double l = tid < EB ? sums[tid] : 0.0;
+#pragma unroll
+    for (int o = kJoinExperts / 2; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    sums[tid] = l;
+  }
   if (tid == 0) {
-    double l = 0.0;
-    for (int i = 0; i < EB; ++i) l += sums[i];
+    double l = sums[0];
     __hip_atomic_store(part + blockIdx.x, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
     if (last) {
