@@ -13,11 +13,12 @@
 // the n-th largest sample, T, is a lower bound of the n-th largest element.  Only the n threads
 // whose sample is at least T can hold an element above it; their elements alone are read again,
 // from the cache, and those of at least T (n and a few) are ranked.  Elements compare as one
-// 64-bit key of value and index, so equal values go to the lowest index, whatever their number.
+// 64-bit key of value and index, so equal values go to the lowest index, whatever their number
+// (the samples as a key of value and granule: a bound on elements all the same).
 //
 // A token outside [0, V) or equal to `ignored` leaves its row unread: zeros, and -1 as top ids.
 // A row of -inf alone has logp -inf, entropy 0 and no gradient.
-#include "common.h"
+#include "wave_ops.h"
 
 namespace hetu {
 
@@ -34,14 +35,14 @@ constexpr float kFloor2 = -200.f;
 // v_exp_f32: results below 2^-126 are 0, which sums of at least 1 do not feel
 __device__ __forceinline__ float exp2_(float t) { return __builtin_amdgcn_exp2f(t); }
 
-__device__ __forceinline__ Lse lse_join(const Lse& a, const Lse& b) {
+// joins the results of G lanes (aligned, a power of two): the largest first, then two plain sums
+__device__ __forceinline__ Lse lse_join(Lse a, int G) {
+#pragma clang fp contract(off)   // a product fused into one lane's sum would leave the lanes unequal
   Lse r;
-  r.m = fmaxf(a.m, b.m);
-  const float sh = shift_of(r.m);
-  const float da = (a.m - sh) * kLog2e, db = (b.m - sh) * kLog2e;
-  const float ea = exp2_(da), eb = exp2_(db);
-  r.s = a.s * ea + b.s * eb;
-  r.u = ea * (a.u + fmaxf(da, kFloor2) * a.s) + eb * (b.u + fmaxf(db, kFloor2) * b.s);
+  r.m = group_max(a.m, G);
+  const float d = (a.m - shift_of(r.m)) * kLog2e, e = exp2_(d);
+  r.s = group_sum(a.s * e, G);
+  r.u = group_sum(e * (a.u + fmaxf(d, kFloor2) * a.s), G);
   return r;
 }
 
@@ -91,13 +92,13 @@ struct Row {
   }
 };
 
-// value (larger first) and index (smaller first) as one number; NaN orders as -inf
-__device__ __forceinline__ uint64_t key_of(float v, int e) {
+// value (larger first) and index (smaller first) as one number, never 0; NaN orders as -inf
+__device__ __forceinline__ unsigned order_of(float v) {
   v = v != v ? -INFINITY : v + 0.f;                      // -0 is 0
   const unsigned b = __float_as_uint(v);
-  const unsigned o = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-  return ((uint64_t)o << 32) | (unsigned)~e;
+  return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ __forceinline__ uint64_t key_of(float v, int e) { return ((uint64_t)order_of(v) << 32) | (unsigned)~e; }
 __device__ __forceinline__ float key_value(uint64_t key) {
   const unsigned o = (unsigned)(key >> 32);
   return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
@@ -138,30 +139,42 @@ __device__ __forceinline__ void lse_take(Lse& a, int& best, const float (&v)[U][
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
                                                       const int64_t* __restrict__ ids, int V, int n, int64_t ignored,
-                                                      float* __restrict__ out, float* __restrict__ stats,
-                                                      int64_t* __restrict__ top) {
-  constexpr int VE = Vec<T>::N, U = 4;              // granules under way at once
+                                                      float* __restrict__ out, int64_t* __restrict__ top) {
+  constexpr int VE = Vec<T>::N, U = 4, NW = NT / 64;
   constexpr int NG = TOP ? (NT < 256 ? NT : 256) : 1, PER = TOP ? NT / NG : 1;   // groups of threads that give a sample
   constexpr int CAND = NT < 256 ? 512 : 1024;       // candidates kept in LDS; more take the slow way
-  __shared__ Lse part[NT / 64];
+  __shared__ Lse part[NW];
   __shared__ uint64_t keys[NG], cand[TOP ? CAND : 1], bound;
   __shared__ int flagged[NG], n_flagged, n_cand;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
+  float* o = out + row * (4 + n);
+  const Row<T> r(logits + row * stride, V);
+  int j = r.f0 + tid;
+  // with few rows the first loads do not wait for the token: one latency less
+  const bool ahead = NT > 256 && j + (U - 1) * NT < r.f1;
+  Raw q[U];
+  if (ahead) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = r.raw(j + u * NT);
+  }
   const int64_t t = ids[row];
-  float* o = out + row * (2 + n);
   if (t < 0 || t >= V || t == ignored) {
-    for (int i = tid; i < 2 + n; i += NT) o[i] = 0.f;
+    for (int i = tid; i < 4 + n; i += NT) o[i] = 0.f;
     for (int i = tid; i < n; i += NT) top[row * n + i] = -1;
-    if (tid < 2) stats[row * 2 + tid] = 0.f;
     return;
   }
-  const Row<T> r(logits + row * stride, V);
+  const float xt = to_f(r.x[t]);
   Lse a = {-INFINITY, 0.f, 0.f};
   int best = -1;
-  int j = r.f0 + tid;
+  if (ahead) {
+    float v[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) unpack(q[u], v[u]);
+    lse_take<U, VE, TOP>(a, best, v, j, NT);
+    j += U * NT;
+  }
   for (; j + (U - 1) * NT < r.f1; j += U * NT) {
-    Raw q[U];
     float v[U][VE];
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = r.raw(j + u * NT);
@@ -169,40 +182,32 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     for (int u = 0; u < U; ++u) unpack(q[u], v[u]);
     lse_take<U, VE, TOP>(a, best, v, j, NT);
   }
-  for (; j < r.f1; j += NT) {
-    float v[1][VE];
-    unpack(r.raw(j), v[0]);
-    lse_take<1, VE, TOP>(a, best, v, j, NT);
-  }
-  if ((tid == 0 && r.has_head()) || (tid == NT - 1 && r.has_tail())) {
-    float v[1][VE];
-    if (tid == 0 && r.has_head()) {
-      r.load(0, v[0]);
-      lse_take<1, VE, TOP>(a, best, v, 0, NT);
-    }
-    if (tid == NT - 1 && r.has_tail()) {
-      r.load(r.ng - 1, v[0]);
-      lse_take<1, VE, TOP>(a, best, v, r.ng - 1, NT);
-    }
-  }
-  // this thread's largest element, for the selection below
-  uint64_t mine = 0;
-  if (TOP && best >= 0) {
-    float v[VE];
-    r.load(best, v);
-    const int e0 = best * VE - r.off;
+  if (j < r.f1) {                     // fewer than U are left: the others' places hold -inf
+    float v[U - 1][VE];
 #pragma unroll
-    for (int k = 0; k < VE; ++k) {
-      const uint64_t key = key_of(v[k], e0 + k);
-      if (e0 + k >= 0 && e0 + k < V && key > mine) mine = key;
-    }
-  }
+    for (int u = 0; u < U - 1; ++u) q[u] = r.raw(j + u * NT < r.f1 ? j + u * NT : j);
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) {
-    const Lse b = {__shfl_xor(a.m, s, 64), __shfl_xor(a.s, s, 64), __shfl_xor(a.u, s, 64)};
-    a = lse_join(a, b);
+    for (int u = 0; u < U - 1; ++u) {
+      unpack(q[u], v[u]);
+#pragma unroll
+      for (int k = 0; k < VE; ++k) v[u][k] = j + u * NT < r.f1 ? v[u][k] : -INFINITY;
+    }
+    lse_take<U - 1, VE, TOP>(a, best, v, j, NT);
   }
-  if (NT > 64 && (tid & 63) == 0) part[tid >> 6] = a;
+  if (tid == 0 && r.has_head()) {
+    float v[1][VE];
+    r.load(0, v[0]);
+    lse_take<1, VE, TOP>(a, best, v, 0, NT);
+  }
+  if (tid == NT - 1 && r.has_tail()) {
+    float v[1][VE];
+    r.load(r.ng - 1, v[0]);
+    lse_take<1, VE, TOP>(a, best, v, r.ng - 1, NT);
+  }
+  uint64_t mine = 0;                  // this thread's sample; 0: it has no element
+  if (TOP && best >= 0) mine = key_of(a.m, best);
+  a = lse_join(a, 64);
+  if (NW > 1 && (tid & 63) == 0) part[tid >> 6] = a;
   if (TOP) {
 #pragma unroll
     for (int s = 1; s < PER; s <<= 1) {
@@ -213,35 +218,43 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     if (tid == 0) { n_flagged = 0; n_cand = 0; }
   }
   __syncthreads();
-  if (NT > 64) {
-    a = part[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) a = lse_join(a, part[w]);
-  }
+  if (NW > 1) a = lse_join(part[tid & (NW - 1)], NW);
   const bool empty = a.m == -INFINITY && a.s == 0.f;
   const float log2s = log2f(a.s), logs = log2s * kLn2;
-  if (tid == 0) {
-    const float xt = to_f(r.x[t]);
+  if (tid == NT - 1) {
     o[0] = empty ? -INFINITY : (xt - a.m) - logs;
     o[1] = empty ? 0.f : (log2s - a.u / a.s) * kLn2;
-    stats[row * 2] = a.m;
-    stats[row * 2 + 1] = log2s;
+    o[2 + n] = a.m;
+    o[3 + n] = log2s;
   }
   if constexpr (TOP) {
     // the n-th largest sample, bit by bit from the highest: the largest key that n samples reach (0
     // where fewer than n threads have an element: then all are candidates)
     if (tid < 64) {
       constexpr int Q = NG / 64;
+      unsigned hi[Q];
       uint64_t k[Q], b = 0;
+      unsigned bh = 0;
+      int reach = 0;
 #pragma unroll
-      for (int q = 0; q < Q; ++q) k[q] = keys[tid + q * 64];
-      for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t c = b | (1ull << bit);
-        int reach = 0;
+      for (int q = 0; q < Q; ++q) {
+        k[q] = keys[tid + q * 64];
+        hi[q] = (unsigned)(k[q] >> 32);
+      }
+      for (int bit = 31; bit >= 0 && reach != n; --bit) {          // by the values,
+        const unsigned c = bh | (1u << bit);
+        reach = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(hi[q] >= c));
+        if (reach >= n) bh = c;
+      }
+      b = (uint64_t)bh << 32;
+      for (int bit = 31; bit >= 0 && reach != n; --bit) {          // and where they tie by the granules
+        const uint64_t c = b | (1u << bit);
+        reach = 0;
 #pragma unroll
         for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(k[q] >= c));
         if (reach >= n) b = c;
-        if (reach == n) break;           // these n are the ones: any bound between them and the next will do
       }
       if (tid == 0) bound = b;
     }
@@ -250,15 +263,16 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     if (tid < NG && keys[tid] != 0 && keys[tid] >= least) flagged[atomicAdd(&n_flagged, 1)] = tid;
     __syncthreads();
     // granules of a flagged group: its threads' whole ones, then the head or tail that is theirs
-    const int J = r.f1 > r.f0 ? (r.f1 - r.f0 + NT - 1) / NT * PER : 0, todo = n_flagged * (J + 1);
+    const int J = r.f1 > r.f0 ? (r.f1 - r.f0 + NT - 1) / NT * PER : 0;
+    const int bits = 32 - __clz(J), todo = n_flagged << bits;      // J + 1 <= 1 << bits
     for (int i = tid; i < todo; i += NT) {
-      const int f = flagged[i / (J + 1)], jj = i % (J + 1);
+      const int f = flagged[i >> bits], jj = i & ((1 << bits) - 1);
       int j = r.f0 + (jj / PER) * NT + f * PER + jj % PER;
       if (jj == J) {
         if (f == 0 && r.has_head()) j = 0;
         else if (f == NG - 1 && r.has_tail()) j = r.ng - 1;
         else continue;
-      } else if (j >= r.f1) {
+      } else if (jj > J || j >= r.f1) {
         continue;
       }
       float v[VE];
@@ -266,10 +280,9 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
       const int e0 = j * VE - r.off;
 #pragma unroll
       for (int k = 0; k < VE; ++k) {
-        const uint64_t key = key_of(v[k], e0 + k);
-        if (e0 + k >= 0 && e0 + k < V && key >= least) {
+        if (e0 + k >= 0 && e0 + k < V && key_of(v[k], j) >= least) {
           const int at = atomicAdd(&n_cand, 1);
-          if (at < CAND) cand[at] = key;
+          if (at < CAND) cand[at] = key_of(v[k], e0 + k);
         }
       }
     }
@@ -328,7 +341,6 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
                                                                    const int64_t* __restrict__ ids, int V, int n,
                                                                    int64_t ignored, int chunks,
                                                                    const float* __restrict__ out,
-                                                                   const float* __restrict__ stats,
                                                                    const int64_t* __restrict__ top,
                                                                    const float* __restrict__ grad, T* __restrict__ dx) {
   constexpr int NT = kBwdThreads, VE = Vec<T>::N, U = kBwdU;
@@ -338,7 +350,8 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
   const int chunk = at % chunks;
   const int64_t t = ids[row];
   T* d = dx + row * (int64_t)V;
-  const float m = stats[row * 2], log2s = stats[row * 2 + 1];
+  const float* o = out + row * (4 + n);
+  const float m = o[2 + n], log2s = o[3 + n];
   const bool dead = t < 0 || t >= V || t == ignored || (m == -INFINITY && log2s == -INFINITY);
   const Row<T> r(logits + row * stride, V), w(d, V);
   const float* g = grad + row * (2 + n);
@@ -347,7 +360,7 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
     all = g[0];
     for (int i = 0; i < n; ++i) all += g[2 + i];
     gh = g[1] * kLn2;
-    all += g[1] * out[row * (2 + n) + 1];
+    all += g[1] * o[1];
   }
   const float sh = shift_of(m);
   const auto slope = [&](float x) {
@@ -422,9 +435,9 @@ using namespace hetu;
 
 template <typename T>
 static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n, int64_t ignored,
-                       float* out, float* stats, int64_t* top, hipStream_t st) {
+                       float* out, int64_t* top, hipStream_t st) {
 #define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), dim3((unsigned)R), dim3(NT), 0, st, \
-                                       (const T*)logits, stride, ids, V, n, ignored, out, stats, top)
+                                       (const T*)logits, stride, ids, V, n, ignored, out, top)
   const int64_t bytes = (int64_t)V * sizeof(T);
   if (bytes <= 4096) { if (n) GO(64, true); else GO(64, false); }
   else if (bytes >= 32768 && R <= 512) { if (n) GO(1024, true); else GO(1024, false); }
@@ -432,19 +445,21 @@ static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, i
 #undef GO
 }
 
+// out: a row of 4 + n: logp, entropy, the n largest log probabilities, then the row's maximum and
+// the base-2 log of its sum for the backward pass
 HETU_API int hetu_token_logprob(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n,
-                                int64_t ignored, float* out, float* stats, int64_t* top, int is_bf16,
+                                int64_t ignored, float* out, int64_t* top, int is_bf16,
                                 hipStream_t st) {
   if (R <= 0) return 0;
   if (V < 1 || n < 0 || n > kMaxTop || n > V || R > 0x7fffffff) return (int)hipErrorInvalidValue;
-  if (is_bf16) launch_fwd<bf16>(logits, stride, ids, R, V, n, ignored, out, stats, top, st);
-  else launch_fwd<float>(logits, stride, ids, R, V, n, ignored, out, stats, top, st);
+  if (is_bf16) launch_fwd<bf16>(logits, stride, ids, R, V, n, ignored, out, top, st);
+  else launch_fwd<float>(logits, stride, ids, R, V, n, ignored, out, top, st);
   HETU_LAUNCH_CHECK();
   return 0;
 }
 
 HETU_API int hetu_token_logprob_bwd(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n,
-                                    int64_t ignored, const float* out, const float* stats, const int64_t* top,
+                                    int64_t ignored, const float* out, const int64_t* top,
                                     const float* grad, void* dx, int is_bf16, hipStream_t st) {
   if (R <= 0) return 0;
   const int VE = is_bf16 ? 8 : 4;
@@ -452,9 +467,9 @@ HETU_API int hetu_token_logprob_bwd(const void* logits, int64_t stride, const in
   if (V < 1 || n < 0 || n > kMaxTop || n > V || R * chunks > 0x7fffffff) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)(R * chunks)), block(kBwdThreads);
   if (is_bf16)
-    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, (int)chunks, out, stats, top, grad, (bf16*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, (int)chunks, out, top, grad, (bf16*)dx);
   else
-    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, (int)chunks, out, stats, top, grad, (float*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, (int)chunks, out, top, grad, (float*)dx);
   HETU_LAUNCH_CHECK();
   return 0;
 }

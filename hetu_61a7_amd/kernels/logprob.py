@@ -13,26 +13,38 @@ MAX_TOP = 64
 
 
 class TokenLogProb(object):
-    """Result of ``token_logprob`` for logits [..., V]: ``logp`` [...] and ``entropy`` [...] and
-    ``top_logp`` [..., top] (views of ``out``, fp32 [..., 2 + top]), ``top_ids`` [..., top]
-    (int64), and ``stats`` [..., 2], each row's maximum and base-2 log of its sum, for the
-    backward pass."""
-    __slots__ = ('out', 'stats', 'top_ids')
+    """Result of ``token_logprob`` for logits [..., V]: ``logp`` [...], ``entropy`` [...] and
+    ``top_logp`` [..., top], all columns of ``out`` (fp32 [..., 2 + top]); ``top_ids`` [..., top]
+    (int64); ``stats`` [..., 2], each row's maximum and base-2 log of its sum, for the backward
+    pass.  The fp32 parts are views of one buffer [..., 4 + top]."""
+    __slots__ = ('buffer', 'top_ids')
 
-    def __init__(self, out, stats, top_ids):
-        self.out, self.stats, self.top_ids = out, stats, top_ids
+    def __init__(self, buffer, top_ids):
+        self.buffer, self.top_ids = buffer, top_ids
+
+    @property
+    def top(self):
+        return self.buffer.shape[-1] - 4
+
+    @property
+    def out(self):
+        return self.buffer[..., :-2]
+
+    @property
+    def stats(self):
+        return self.buffer[..., -2:]
 
     @property
     def logp(self):
-        return self.out[..., 0]
+        return self.buffer[..., 0]
 
     @property
     def entropy(self):
-        return self.out[..., 1]
+        return self.buffer[..., 1]
 
     @property
     def top_logp(self):
-        return self.out[..., 2:]
+        return self.buffer[..., 2:-2]
 
 
 def _operands(name, logits, ids, top):
@@ -71,18 +83,17 @@ def token_logprob(logits, ids, top=0, ignored_index=-1):
     are 0, top_ids -1.  A row with nothing above -inf has logp and top_logp -inf and entropy 0.
     A NaN or +inf makes its row NaN."""
     x, ids, lead, R, V = _operands('token_logprob', logits, ids, top)
-    out = _NA.empty(lead + (2 + top,), dtype=torch.float32, device=x.device)
-    stats = _NA.empty(lead + (2,), dtype=torch.float32, device=x.device)
-    top_ids = _NA.empty(lead + (top,), dtype=torch.int64, device=x.device)
+    r = TokenLogProb(_NA.empty(lead + (4 + top,), dtype=torch.float32, device=x.device),
+                     _NA.empty(lead + (top,), dtype=torch.int64, device=x.device))
     if R == 0:
-        return TokenLogProb(out, stats, top_ids)
+        return r
     if native(x):
         check_device(x, 'token_logprob')
-        f = fn('hetu_token_logprob', [P, I64, P, I64, I32, I32, I64, P, P, P, I32, P])
-        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, int(ignored_index), out.data_ptr(),
-                stats.data_ptr(), top_ids.data_ptr(), is_bf16(x), stream_ptr()), 'token_logprob')
+        f = fn('hetu_token_logprob', [P, I64, P, I64, I32, I32, I64, P, P, I32, P])
+        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, ignored_index, r.buffer.data_ptr(),
+                r.top_ids.data_ptr(), is_bf16(x), stream_ptr()), 'token_logprob')
         record_native('token_logprob')
-        return TokenLogProb(out, stats, top_ids)
+        return r
     xf = x.float()
     valid = (ids >= 0) & (ids < V) & (ids != ignored_index)
     m = xf.amax(1, keepdim=True)
@@ -97,26 +108,25 @@ def token_logprob(logits, ids, top=0, ignored_index=-1):
         order = torch.where(torch.isnan(xf), torch.full_like(xf, -math.inf), xf)
         idx = torch.sort(order, dim=1, descending=True, stable=True)[1][:, :top]
         res = torch.cat([res, z.gather(1, idx) - logs], 1)
-        top_ids.copy_(torch.where(valid[:, None], idx, torch.full_like(idx, -1)).reshape(top_ids.shape))
+        r.top_ids.copy_(torch.where(valid[:, None], idx, torch.full_like(idx, -1)).reshape(r.top_ids.shape))
     res[empty] = -math.inf
     res[empty, 1] = 0.0
     res[~valid] = 0.0
-    out.copy_(res.reshape(out.shape))
     st = torch.cat([m, torch.log2(s)], 1)
     st[~valid] = 0.0
-    stats.copy_(st.reshape(stats.shape))
-    return TokenLogProb(out, stats, top_ids)
+    r.buffer.copy_(torch.cat([res, st], 1).reshape(r.buffer.shape))
+    return r
 
 
 def token_logprob_backward(logits, ids, fwd, grad, ignored_index=-1):
     """d logits (contiguous, of the logits' type) from ``grad`` [..., 2 + top], the gradient of
     ``fwd.out``: of logp, of the entropy and of each of ``fwd``'s alternatives.  ``fwd`` is what
     ``token_logprob`` gave for the same logits, ids and ignored_index."""
-    top = fwd.out.shape[-1] - 2
+    top = fwd.top
     x, ids, lead, R, V = _operands('token_logprob_backward', logits, ids, top)
-    if tuple(fwd.out.shape) != lead + (2 + top,) or grad.numel() != fwd.out.numel() or grad.device != x.device:
-        raise ValueError('token_logprob_backward: logits %s, forward %s, gradient %s'
-                         % (tuple(logits.shape), tuple(fwd.out.shape), tuple(grad.shape)))
+    if tuple(fwd.buffer.shape) != lead + (4 + top,) or grad.numel() != R * (2 + top) or grad.device != x.device:
+        raise ValueError('token_logprob_backward: logits %s, forward of %s, gradient %s'
+                         % (tuple(logits.shape), tuple(fwd.buffer.shape[:-1]), tuple(grad.shape)))
     if grad.dtype != torch.float32 or not grad.is_contiguous():
         from .moe import _dc
         grad = _dc(grad, torch.float32)
@@ -125,10 +135,10 @@ def token_logprob_backward(logits, ids, fwd, grad, ignored_index=-1):
         return dx
     if native(x):
         check_device(x, 'token_logprob_backward')
-        f = fn('hetu_token_logprob_bwd', [P, I64, P, I64, I32, I32, I64, P, P, P, P, P, I32, P])
-        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, int(ignored_index), fwd.out.data_ptr(),
-                fwd.stats.data_ptr(), fwd.top_ids.data_ptr(), grad.data_ptr(), dx.data_ptr(), is_bf16(x),
-                stream_ptr()), 'token_logprob_bwd')
+        f = fn('hetu_token_logprob_bwd', [P, I64, P, I64, I32, I32, I64, P, P, P, P, I32, P])
+        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, ignored_index, fwd.buffer.data_ptr(),
+                fwd.top_ids.data_ptr(), grad.data_ptr(), dx.data_ptr(), is_bf16(x), stream_ptr()),
+              'token_logprob_bwd')
         record_native('token_logprob_bwd')
         return dx
     g, o = grad.reshape(R, 2 + top), fwd.out.reshape(R, 2 + top)

@@ -233,7 +233,7 @@ def test_refusals():
     with pytest.raises(ValueError):
         K.token_logprob(big, torch.zeros(1, dtype=torch.int64), 65)
     r = K.token_logprob(x, ids, 2)
-    for a in ((x, ids, r, torch.zeros(4, 3)), (x[:2], ids[:2], r, torch.zeros(2, 4))):
+    for a in ((x, ids, r, torch.zeros(4, 3)), (x[:2], ids[:2], r, torch.zeros(2, 4)), (x[:, :1], ids, r, torch.zeros(4, 4))):
         with pytest.raises(ValueError):
             K.token_logprob_backward(*a)
     with pytest.raises(ValueError):
@@ -278,7 +278,7 @@ def test_op_values_and_gradients(device, graph):
     for _ in range(6 if graph else 1):
         out = ex.run('train', feed_dict=feed, convert_to_numpy_ret_vals=True)
         lp, e, t, i, d = [torch.from_numpy(np.asarray(o)) for o in out]
-        r = K.TokenLogProb(torch.cat([lp[:, None], e[:, None], t], 1), None, i)
+        r = K.TokenLogProb(torch.cat([lp[:, None], e[:, None], t, t[:, :2]], 1), i)
         _check(x, ids, top, torch.float32, r, d, w)
 
 
