@@ -439,8 +439,11 @@ static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, i
 #define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), dim3((unsigned)R), dim3(NT), 0, st, \
                                        (const T*)logits, stride, ids, V, n, ignored, out, top)
   const int64_t bytes = (int64_t)V * sizeof(T);
+  // a wave a row up to 4 KB; 1024 threads for long rows that are few, or that have alternatives to
+  // find (a thread's elements are read again: 1000 x 131072 top 20 63 us, with 256 threads 71); 256
+  // threads else (8192 x 30522 117 us, with 128 130, with 512 124)
   if (bytes <= 4096) { if (n) GO(64, true); else GO(64, false); }
-  else if (bytes >= 32768 && R <= 512) { if (n) GO(1024, true); else GO(1024, false); }
+  else if (bytes >= 32768 && (R <= 512 || n)) { if (n) GO(1024, true); else GO(1024, false); }
   else { if (n) GO(256, true); else GO(256, false); }
 #undef GO
 }

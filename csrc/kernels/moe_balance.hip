@@ -6,7 +6,8 @@
 //   dx_{t,e} = g p_{t,e} (w_e - sum_f p_{t,f} w_f)       (the counts carry no gradient)
 //
 // A row of E logits is held by a group of G lanes (a power of two, at most a wave) in registers:
-// lane l of a group holds elements (j G + l) V + k for j < NJ, k < V, V elements a load.  Column
+// lane l of a group holds elements (j G + l) V + k for j < NJ, k < V, V elements a load.  G, V and
+// NJ are known at compile time, so that the exchanges of several rows' reductions interleave.  Column
 // sums stay in the lanes' registers over all rows of a block, join by shuffles and LDS, and go to
 // a row of partial sums a block; one block adds those up in a fixed order.  No atomics on floats:
 // the same inputs give the same bits.
@@ -17,113 +18,179 @@ namespace hetu {
 constexpr int kBlThreads = 256;
 constexpr int kMaxExperts = 1024;
 
-// validity of token t from a mask of 1-byte (0), fp32 (1), bf16 (2), int64 (3) or int32 (4) values
-__device__ __forceinline__ bool token_on(const void* valid, int kind, int64_t t) {
-  if (!valid) return true;
-  switch (kind) {
-    case 0: return ((const unsigned char*)valid)[t] != 0;
-    case 1: return ((const float*)valid)[t] != 0.f;
-    case 2: return (((const unsigned short*)valid)[t] & 0x7FFFu) != 0;
-    case 3: return ((const int64_t*)valid)[t] != 0;
-    default: return ((const int*)valid)[t] != 0;
+// validity of tokens t, t + step, .. (U of them, those below t1) from a mask of 1-byte (0), fp32
+// (1), bf16 (2), int64 (3) or int32 (4) values
+template <int U, typename M>
+__device__ __forceinline__ void mask_on(const M* mask, M bits, int64_t t, int64_t step, int64_t t1, bool (&on)[U]) {
+  M v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = mask[t + u * step < t1 ? t + u * step : t1 - 1];
+#pragma unroll
+  for (int u = 0; u < U; ++u) on[u] = t + u * step < t1 && (v[u] & bits) != 0;
+}
+template <int U>
+__device__ __forceinline__ void tokens_on(const void* valid, int kind, int64_t t, int64_t step, int64_t t1, bool (&on)[U]) {
+  if (!valid) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) on[u] = t + u * step < t1;
+  } else if (kind == 0) {
+    mask_on<U, unsigned char>((const unsigned char*)valid, 0xFF, t, step, t1, on);
+  } else if (kind == 2) {
+    mask_on<U, unsigned short>((const unsigned short*)valid, 0x7FFF, t, step, t1, on);     // -0 is 0
+  } else if (kind == 3) {
+    mask_on<U, uint64_t>((const uint64_t*)valid, ~0ull, t, step, t1, on);
+  } else {
+    mask_on<U, unsigned>((const unsigned*)valid, kind == 1 ? 0x7FFFFFFFu : ~0u, t, step, t1, on);
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_n(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) v[0] = to_f(p[0]);
-  else load_vec<T>(p, v);
-}
 template <typename T, int V>
 __device__ __forceinline__ void store_n(T* p, const float (&v)[V]) {
   if constexpr (V == 1) p[0] = from_f<T>(v[0]);
   else store_vec<T>(p, v);
 }
 
-// the lane's elements of row x, -inf beyond E
-template <typename T, int V, int NJ>
-__device__ __forceinline__ void row_load(const T* x, int E, int G, int lane, float (&p)[NJ * V]) {
+// A lane's elements of a row as they are in memory: converted when they are used, so that loads
+// can be under way across other work.  V = 1, or the 4 fp32 or 8 bf16 of 16 bytes.  Lanes beyond E
+// hold the row's first elements again: they leave the maximum as it is, and are left out of sums.
+template <typename T, int V, int NJ, int G>
+struct RowRaw {
+  typedef unsigned Q4 __attribute__((ext_vector_type(4)));
+  Q4 q[V == 1 ? 1 : NJ];
+  T s[V == 1 ? NJ : 1];
+  __device__ __forceinline__ void load(const T* x, int E, int lane) {
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int e = (j * G + lane) * V;
-    float v[V];
-    if (e < E) {
-      load_n<T, V>(x + e, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = -INFINITY;
+    for (int j = 0; j < NJ; ++j) {
+      int e = (j * G + lane) * V;
+      e = e < E ? e : 0;
+      if constexpr (V == 1) s[j] = x[e];
+      else q[j] = *reinterpret_cast<const Q4*>(x + e);
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) p[j * V + k] = v[k];
   }
+  __device__ __forceinline__ void unpack(float (&p)[NJ * V]) const {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if constexpr (V == 1) p[j] = to_f(s[j]);
+        else if constexpr (V == 4) p[j * V + k] = __uint_as_float(q[j][k]);
+        else p[j * V + k] = __uint_as_float(k & 1 ? q[j][k >> 1] & 0xffff0000u : q[j][k >> 1] << 16);
+      }
+  }
+};
+
+// exponentials of U rows in place and the reciprocals of their sums (v_rcp_f32, off by a unit)
+template <int U, int V, int NJ, int G>
+__device__ __forceinline__ void rows_exp(int E, int lane, float (&p)[U][NJ * V], float (&inv)[U]) {
+  float m[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    m[u] = p[u][0];
+#pragma unroll
+    for (int i = 1; i < NJ * V; ++i) m[u] = fmaxf(m[u], p[u][i]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) m[u] = group_max(m[u], G);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float part = 0.f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        p[u][j * V + k] = __expf(p[u][j * V + k] - m[u]);
+        part += p[u][j * V + k];
+      }
+      s += (j * G + lane) * V < E ? part : 0.f;
+    }
+    inv[u] = s;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) inv[u] = __builtin_amdgcn_rcpf(group_sum(inv[u], G));
 }
 
-// exponentials in place, 0 beyond E, and the reciprocal of their sum over the row
-template <int N>
-__device__ __forceinline__ float row_exp(int G, float (&p)[N]) {
-  float m = p[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, p[i]);
-  m = group_max(m, G);
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = __expf(p[i] - m);
-    s += p[i];
-  }
-  return 1.f / group_sum(s, G);
-}
+// Partial sums of block b: psum [b][E], counts [b][E + 1] (the last: valid tokens).  A group takes
+// U rows at a time: the next U rows' loads and the validity of those after them are under way
+// while these are summed.
+constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;
 
-// Partial sums of block b: psum [b][E], counts [b][E + 1] (the last: valid tokens).  U rows a
-// group are under way at once: their loads and the exchanges of their two reductions overlap.
-template <typename T, int V, int NJ>
-__global__ void __launch_bounds__(kBlThreads) balance_part_k(const T* __restrict__ x, int64_t stride, int64_t T_, int E,
-                                                             int G, const int64_t* __restrict__ idx, int k,
-                                                             const void* valid, int kind, int64_t rows,
-                                                             float* __restrict__ psum, int* __restrict__ pcnt,
-                                                             unsigned* __restrict__ ticket) {
-  constexpr int N = NJ * V, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1);
-  __shared__ float cols[4][kMaxExperts];
-  __shared__ int hist[kMaxExperts + 1];
-  const int tid = threadIdx.x, lane = tid & (G - 1), group = tid / G, groups = kBlThreads / G;
+template <typename T, int V, int NJ, int G>
+__global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restrict__ x, int64_t stride, int64_t T_,
+                                                               int E, const int64_t* __restrict__ idx, int k,
+                                                               const void* valid, int kind, int64_t rows,
+                                                               float* __restrict__ psum, int* __restrict__ pcnt,
+                                                               unsigned* __restrict__ ticket) {
+  constexpr int N = NJ * V, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1), CU = 4, groups = kPartThreads / G;
+  constexpr int64_t step = groups * U;
+  extern __shared__ int lds[];
+  int* hist = lds;                                       // [E + 1]
+  float* cols = reinterpret_cast<float*>(lds + E + 1);   // [kPartWaves][E]
+  const int tid = threadIdx.x, lane = tid & (G - 1), group = tid / G;
   const int64_t t0 = (int64_t)blockIdx.x * rows, t1 = t0 + rows < T_ ? t0 + rows : T_;
   if (blockIdx.x == 0 && tid == 0) *ticket = 0;       // for the joining launch
-  for (int e = tid; e <= E; e += kBlThreads) hist[e] = 0;
+  for (int e = tid; e <= E; e += kPartThreads) hist[e] = 0;
   __syncthreads();
+  RowRaw<T, V, NJ, G> raw[U];
+  const T *base = x + t0 * stride, *at = x + (t0 + group) * stride;
+  const int64_t between = groups * stride;
+  const auto load = [&](const bool (&on)[U]) {          // not valid: the row of t0 in its place, unused
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(on[u] ? at + u * between : base, E, lane);
+  };
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  // the choices, one a thread: (token, choice) advances by 256 choices without a division
+  int count = 0;
+  bool on[U], next[U];
+  int64_t t = t0 + group;
+  if (t < t1) {
+    tokens_on<U>(valid, kind, t, groups, t1, on);
+    load(on);
+    tokens_on<U>(valid, kind, t + step, groups, t1, next);
+  }
+  // the choices, one a thread, CU of them under way: (token, choice) advances by the block's
+  // threads without a division
   {
-    const int dt = kBlThreads / k, dc = kBlThreads - dt * k;
-    int64_t t = t0 + tid / k;
+    const int dt = kPartThreads / k, dc = kPartThreads - dt * k;
+    int64_t tc = t0 + tid / k;
     int c = tid % k;
-    while (t < t1) {
-      if (token_on(valid, kind, t)) {
-        const int64_t e = idx[t * k + c];
-        if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
+    while (tc < t1) {
+      int64_t e[CU];
+      bool in[CU][1];
+#pragma unroll
+      for (int u = 0; u < CU; ++u) {
+        e[u] = tc < t1 ? idx[tc * k + c] : -1;
+        tokens_on<1>(valid, kind, tc, 0, t1, in[u]);
+        tc += dt;
+        c += dc;
+        if (c >= k) { c -= k; ++tc; }
       }
-      t += dt;
-      c += dc;
-      if (c >= k) { c -= k; ++t; }
+#pragma unroll
+      for (int u = 0; u < CU; ++u)
+        if (in[u][0] && e[u] >= 0 && e[u] < E) atomicAdd(&hist[e[u]], 1);
     }
   }
-  int count = 0;
-  for (int64_t t = t0 + group; t < t1; t += (int64_t)groups * U) {
-    float p[U][N];
-    bool on[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {      // a token that is not valid: the row of t0 in its place, unused
-      const int64_t tu = t + (int64_t)u * groups;
-      on[u] = tu < t1 && token_on(valid, kind, tu);
-      row_load<T, V, NJ>(x + (on[u] ? tu : t0) * stride, E, G, lane, p[u]);
-      count += on[u];
-    }
+  for (; t < t1; t += step) {
+    float p[U][N], inv[U];
+    bool now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float inv = row_exp<N>(G, p[u]);
+      raw[u].unpack(p[u]);
+      now[u] = on[u];
+      on[u] = next[u];
+    }
+    if (t + step < t1) {
+      at += step * stride;
+      load(on);
+      tokens_on<U>(valid, kind, t + 2 * step, groups, t1, next);
+    }
+    rows_exp<U, V, NJ, G>(E, lane, p, inv);
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += on[u] ? p[u][i] * inv : 0.f;
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += now[u] ? p[u][i] * inv[u] : 0.f;
+      count += now[u];
     }
   }
   if (lane == 0 && count) atomicAdd(&hist[E], count);
@@ -137,14 +204,18 @@ __global__ void __launch_bounds__(kBlThreads) balance_part_k(const T* __restrict
       const int e = (j * G + lane) * V;
       if (e < E) {
 #pragma unroll
-        for (int q = 0; q < V; ++q) cols[tid >> 6][e + q] = acc[j * V + q];
+        for (int q = 0; q < V; ++q) cols[(tid >> 6) * E + e + q] = acc[j * V + q];
       }
     }
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kBlThreads)
-    psum[(int64_t)blockIdx.x * E + e] = (cols[0][e] + cols[1][e]) + (cols[2][e] + cols[3][e]);
-  for (int e = tid; e <= E; e += kBlThreads) pcnt[(int64_t)blockIdx.x * (E + 1) + e] = hist[e];
+  for (int e = tid; e < E; e += kPartThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPartWaves; ++w) s += cols[w * E + e];
+    psum[(int64_t)blockIdx.x * E + e] = s;
+  }
+  for (int e = tid; e <= E; e += kPartThreads) pcnt[(int64_t)blockIdx.x * (E + 1) + e] = hist[e];
 }
 
 // Counts, the weights of the backward pass and the loss from the blocks' sums: EB experts a
@@ -217,13 +288,15 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __re
   }
 }
 
-template <typename T, int V, int NJ>
+// U rows a group at a time
+template <typename T, int V, int NJ, int G>
 __global__ void __launch_bounds__(kBlThreads) balance_bwd_k(const T* __restrict__ x, int64_t stride, int64_t T_, int E,
-                                                            int G, const float* __restrict__ weight,
+                                                            const float* __restrict__ weight,
                                                             const float* __restrict__ g, const void* valid, int kind,
                                                             T* __restrict__ dx) {
-  const int tid = threadIdx.x, lane = tid & (G - 1), group = tid / G, groups = kBlThreads / G;
-  float w[NJ * V];
+  constexpr int N = NJ * V, U = N <= 8 ? 2 : 1, groups = kBlThreads / G;
+  const int tid = threadIdx.x, lane = tid & (G - 1), group = tid / G;
+  float w[N];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int e = (j * G + lane) * V;
@@ -231,30 +304,45 @@ __global__ void __launch_bounds__(kBlThreads) balance_bwd_k(const T* __restrict_
     for (int q = 0; q < V; ++q) w[j * V + q] = e < E ? weight[e + q] : 0.f;
   }
   const float gr = g[0];
-  for (int64_t t = (int64_t)blockIdx.x * groups + group; t < T_; t += (int64_t)gridDim.x * groups) {
-    float p[NJ * V];
-    if (token_on(valid, kind, t)) {
-      row_load<T, V, NJ>(x + t * stride, E, G, lane, p);
-      const float inv = row_exp<NJ * V>(G, p);
-      float dot = 0.f;
+  for (int64_t t = (int64_t)blockIdx.x * groups * U + group; t < T_; t += (int64_t)gridDim.x * groups * U) {
+    RowRaw<T, V, NJ, G> raw[U];
+    float p[U][N], inv[U], dot[U];
+    bool on[U];
+    tokens_on<U>(valid, kind, t, groups, T_, on);
+    bool any = false;
 #pragma unroll
-      for (int i = 0; i < NJ * V; ++i) dot += p[i] * w[i];
-      dot = group_sum(dot, G) * inv;
-      const float c = gr * inv;
+    for (int u = 0; u < U; ++u) any |= on[u];
+    if (any) {
 #pragma unroll
-      for (int i = 0; i < NJ * V; ++i) p[i] = c * p[i] * (w[i] - dot);
-    } else {
+      for (int u = 0; u < U; ++u) {       // one that is not valid: its fellow's row in its place, unused
+        const int64_t tu = on[u] ? t + u * groups : (on[0] ? t : t + (U - 1) * groups);
+        raw[u].load(x + tu * stride, E, lane);
+      }
 #pragma unroll
-      for (int i = 0; i < NJ * V; ++i) p[i] = 0.f;
+      for (int u = 0; u < U; ++u) raw[u].unpack(p[u]);
+      rows_exp<U, V, NJ, G>(E, lane, p, inv);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        dot[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) dot[u] += p[u][i] * w[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) dot[u] = group_sum(dot[u], G) * inv[u];
     }
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int e = (j * G + lane) * V;
-      if (e < E) {
-        float v[V];
+    for (int u = 0; u < U; ++u) {
+      const int64_t tu = t + u * groups;
+      const float c = on[u] ? gr * inv[u] : 0.f;
 #pragma unroll
-        for (int q = 0; q < V; ++q) v[q] = p[j * V + q];
-        store_n<T, V>(dx + t * (int64_t)E + e, v);
+      for (int j = 0; j < NJ; ++j) {
+        const int e = (j * G + lane) * V;
+        if (tu < T_ && e < E) {
+          float v[V];
+#pragma unroll
+          for (int q = 0; q < V; ++q) v[q] = on[u] ? c * p[u][j * V + q] * (w[j * V + q] - dot[u]) : 0.f;
+          store_n<T, V>(dx + tu * (int64_t)E + e, v);
+        }
       }
     }
   }
@@ -279,54 +367,80 @@ static RowPlan plan_rows(int E, int64_t stride, const void* x, const void* y, in
 
 using namespace hetu;
 
-// Rows a block of the partial sums takes: as many blocks as keep the chip's waves busy (4 blocks a
-// CU), but at least 8 rows a group of lanes, for each block costs E partial sums.
+// Rows a block of the partial sums takes: as many blocks as keep the chip's waves busy (4 blocks of 8
+// waves a CU), but at least 8 rows a group of lanes, for each block costs E partial sums.
 constexpr int kMaxParts = 1024;
 static int64_t balance_rows(int64_t T, int G) {
-  const int64_t groups = kBlThreads / G;
+  const int64_t groups = kPartThreads / G;
   int64_t blocks = (T + groups * 8 - 1) / (groups * 8);
   blocks = blocks < 1 ? 1 : (blocks > kMaxParts ? kMaxParts : blocks);
   return (T + blocks - 1) / blocks;
 }
 
-#define BALANCE_CASES(GO)                                                            \
-  if (is_bf16) {                                                                     \
-    if (r.V == 8) { if (r.NJ == 1) GO(bf16, 8, 1); else GO(bf16, 8, 2); }            \
-    else if (r.NJ == 1) GO(bf16, 1, 1); else if (r.NJ == 2) GO(bf16, 1, 2);          \
-    else if (r.NJ == 4) GO(bf16, 1, 4); else if (r.NJ == 8) GO(bf16, 1, 8);          \
-    else GO(bf16, 1, 16);                                                            \
-  } else {                                                                           \
-    if (r.V == 4) { if (r.NJ == 1) GO(float, 4, 1); else if (r.NJ == 2) GO(float, 4, 2); else GO(float, 4, 4); } \
-    else if (r.NJ == 1) GO(float, 1, 1); else if (r.NJ == 2) GO(float, 1, 2);        \
-    else if (r.NJ == 4) GO(float, 1, 4); else if (r.NJ == 8) GO(float, 1, 8);        \
-    else GO(float, 1, 16);                                                           \
+// calls f(V, NJ, G) as compile-time numbers for the plan
+template <int N> struct Const { static constexpr int value = N; };
+template <int V, int NJ, typename F>
+static void with_group(int G, F f) {
+  if constexpr (NJ > 1) f(Const<V>(), Const<NJ>(), Const<64>());
+  else if (G == 1) f(Const<V>(), Const<1>(), Const<1>());
+  else if (G == 2) f(Const<V>(), Const<1>(), Const<2>());
+  else if (G == 4) f(Const<V>(), Const<1>(), Const<4>());
+  else if (G == 8) f(Const<V>(), Const<1>(), Const<8>());
+  else if (G == 16) f(Const<V>(), Const<1>(), Const<16>());
+  else if (G == 32) f(Const<V>(), Const<1>(), Const<32>());
+  else f(Const<V>(), Const<1>(), Const<64>());
+}
+template <int VEC, typename F>      // VEC: elements of 16 bytes
+static void with_plan(const RowPlan& r, F f) {
+  if (r.V == VEC) {
+    if (r.NJ == 1) with_group<VEC, 1>(r.G, f);
+    else if (r.NJ == 2) with_group<VEC, 2>(r.G, f);
+    else if constexpr (VEC == 4) with_group<VEC, 4>(r.G, f);
+  } else if (r.NJ == 1) {
+    with_group<1, 1>(r.G, f);
+  } else if (r.NJ == 2) {
+    with_group<1, 2>(r.G, f);
+  } else if (r.NJ == 4) {
+    with_group<1, 4>(r.G, f);
+  } else if (r.NJ == 8) {
+    with_group<1, 8>(r.G, f);
+  } else {
+    with_group<1, 16>(r.G, f);
   }
+}
 
 // number of 4-byte words of workspace (8-byte aligned) that hetu_moe_balance_fwd needs: each
 // block's sums and counts, the joining blocks' parts of the loss, their ticket
 HETU_API int64_t hetu_moe_balance_ws(int64_t T, int E) {
   if (T < 0 || E < 1 || E > kMaxExperts) return 0;
-  const int64_t groups_least = kBlThreads / 64;
+  const int64_t groups_least = kPartThreads / 64;
   int64_t parts = (T + groups_least * 8 - 1) / (groups_least * 8);
   parts = parts < 1 ? 1 : (parts > kMaxParts ? kMaxParts : parts);
   return 2 * (kMaxExperts / kJoinExperts) + 2 + parts * (2 * E + 1);
 }
 
+// counts: a buffer of E int64, then (as fp32) E weights and the loss
 HETU_API int hetu_moe_balance_fwd(const void* x, int64_t stride, int64_t T, int E, const int64_t* idx, int k,
-                                  const void* valid, int kind, int64_t* counts, float* weight, float* loss, void* ws,
-                                  int is_bf16, hipStream_t st) {
+                                  const void* valid, int kind, int64_t* counts, void* ws, int is_bf16,
+                                  hipStream_t st) {
   if (T < 0 || E < 1 || E > kMaxExperts || k < 1) return (int)hipErrorInvalidValue;
   const RowPlan r = plan_rows(E, stride, x, nullptr, is_bf16 ? 8 : 4);
   const int64_t rows = T > 0 ? balance_rows(T, r.G) : 1;
   const int blocks = T > 0 ? (int)((T + rows - 1) / rows) : 1;
+  float *weight = (float*)(counts + E), *loss = weight + E;
   double* part = (double*)ws;
   unsigned* ticket = (unsigned*)(part + kMaxExperts / kJoinExperts);
   float* psum = (float*)(ticket + 2);
   int* pcnt = (int*)(psum + (int64_t)blocks * E);
-#define GO(TT, VV, JJ) hipLaunchKernelGGL((balance_part_k<TT, VV, JJ>), dim3(blocks), dim3(kBlThreads), 0, st, \
-                                          (const TT*)x, stride, T, E, r.G, idx, k, valid, kind, rows, psum, pcnt, ticket)
-  BALANCE_CASES(GO)
-#undef GO
+  const size_t lds = sizeof(int) * (size_t)(E + 1 + kPartWaves * E);
+  const auto go = [&](auto zero, auto v, auto nj, auto g) {
+    typedef decltype(zero) TT;
+    hipLaunchKernelGGL((balance_part_k<TT, decltype(v)::value, decltype(nj)::value, decltype(g)::value>), dim3(blocks),
+                       dim3(kPartThreads), lds, st, (const TT*)x, stride, T, E, idx, k, valid, kind, rows, psum, pcnt,
+                       ticket);
+  };
+  if (is_bf16) with_plan<8>(r, [&](auto v, auto nj, auto g) { go(bf16(), v, nj, g); });
+  else with_plan<4>(r, [&](auto v, auto nj, auto g) { go(0.f, v, nj, g); });
   HETU_LAUNCH_CHECK();
   int EB = 1;
   while (EB < E && EB < kJoinExperts) EB <<= 1;
@@ -336,18 +450,21 @@ HETU_API int hetu_moe_balance_fwd(const void* x, int64_t stride, int64_t T, int 
   return 0;
 }
 
-HETU_API int hetu_moe_balance_bwd(const void* x, int64_t stride, int64_t T, int E, const float* weight, const float* g,
+HETU_API int hetu_moe_balance_bwd(const void* x, int64_t stride, int64_t T, int E, const float* weight, const float* grad,
                                   const void* valid, int kind, void* dx, int is_bf16, hipStream_t st) {
   if (T <= 0) return 0;
   if (E < 1 || E > kMaxExperts) return (int)hipErrorInvalidValue;
   const RowPlan r = plan_rows(E, stride, x, dx, is_bf16 ? 8 : 4);
-  const int64_t groups = kBlThreads / r.G;
+  const int64_t groups = kBlThreads / r.G * (r.NJ * r.V <= 8 ? 2 : 1);
   const int64_t want = (T + groups - 1) / groups;
   const dim3 grid((unsigned)(want < 2048 ? want : 2048));
-#define GO(TT, VV, JJ) hipLaunchKernelGGL((balance_bwd_k<TT, VV, JJ>), grid, dim3(kBlThreads), 0, st, (const TT*)x, \
-                                          stride, T, E, r.G, weight, g, valid, kind, (TT*)dx)
-  BALANCE_CASES(GO)
-#undef GO
+  const auto go = [&](auto zero, auto v, auto nj, auto g) {
+    typedef decltype(zero) TT;
+    hipLaunchKernelGGL((balance_bwd_k<TT, decltype(v)::value, decltype(nj)::value, decltype(g)::value>), grid,
+                       dim3(kBlThreads), 0, st, (const TT*)x, stride, T, E, weight, grad, valid, kind, (TT*)dx);
+  };
+  if (is_bf16) with_plan<8>(r, [&](auto v, auto nj, auto g) { go(bf16(), v, nj, g); });
+  else with_plan<4>(r, [&](auto v, auto nj, auto g) { go(0.f, v, nj, g); });
   HETU_LAUNCH_CHECK();
   return 0;
 }

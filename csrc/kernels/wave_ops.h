@@ -1,0 +1,57 @@
+// Reductions over aligned groups of lanes of a wave (2, 4, .. 64 lanes; every lane gets the
+// result), by lane exchanges of the vector unit instead of LDS permutes: lanes 1 and 2 apart within
+// a quad, then quads and halves of a row of 16 mirrored, then rows and halves of the wave swapped
+// (v_permlane16_swap, v_permlane32_swap).
+#pragma once
+#include "common.h"
+
+namespace hetu {
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
+}
+
+// joins v with the value of the lane (or of an equal group of lanes) that step O pairs it with:
+// after steps 1, 2, .. G / 2 all lanes of a group of G hold the same
+template <int O, typename F>
+__device__ __forceinline__ unsigned lane_join(unsigned v, F f) {
+  if constexpr (O == 1) return f(v, dpp<0xB1>(v));         // quad_perm 1 0 3 2
+  else if constexpr (O == 2) return f(v, dpp<0x4E>(v));    // quad_perm 2 3 0 1
+  else if constexpr (O == 4) return f(v, dpp<0x141>(v));   // row_half_mirror: the other quad
+  else if constexpr (O == 8) return f(v, dpp<0x140>(v));   // row_mirror: the other half row
+  else if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return f(r[0], r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(r[0], r[1]);
+  }
+}
+
+template <typename F>
+__device__ __forceinline__ unsigned group_join(unsigned v, int G, F f) {
+  if (G > 1) v = lane_join<1>(v, f);
+  if (G > 2) v = lane_join<2>(v, f);
+  if (G > 4) v = lane_join<4>(v, f);
+  if (G > 8) v = lane_join<8>(v, f);
+  if (G > 16) v = lane_join<16>(v, f);
+  if (G > 32) v = lane_join<32>(v, f);
+  return v;
+}
+
+__device__ __forceinline__ float group_max(float v, int G) {
+  return __uint_as_float(group_join(__float_as_uint(v), G, [](unsigned a, unsigned b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+// (v as it is: where the compiler may fuse v's last product into the first sum, lanes differ by a rounding)
+__device__ __forceinline__ float group_sum(float v, int G) {
+#pragma clang fp contract(off)
+  return __uint_as_float(group_join(__float_as_uint(v), G, [](unsigned a, unsigned b) {
+#pragma clang fp contract(off)
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
+}  // namespace hetu

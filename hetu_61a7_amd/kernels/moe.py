@@ -11,6 +11,7 @@ the top-k gate is fused (softmax + top-k + capacity slots + balance terms).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from .. import native_array as _NA
@@ -114,11 +115,29 @@ _VALID_KINDS = {torch.bool: 0, torch.uint8: 0, torch.int8: 0, torch.float32: 1, 
 
 class BalanceLoss(object):
     """Result of ``balance_loss``: ``loss`` fp32 [1], ``counts`` int64 [E], and ``weight`` fp32 [E],
-    d loss / d (sum of the tokens' probabilities of an expert), for the backward pass."""
-    __slots__ = ('loss', 'counts', 'weight')
+    d loss / d (sum of the tokens' probabilities of an expert), for the backward pass: views of
+    one int64 buffer of E counts, then (as fp32) E weights and the loss."""
+    __slots__ = ('buffer', 'experts')
 
-    def __init__(self, loss, counts, weight):
-        self.loss, self.counts, self.weight = loss, counts, weight
+    def __init__(self, buffer, experts):
+        self.buffer, self.experts = buffer, experts
+
+    @property
+    def counts(self):
+        return self.buffer[:self.experts]
+
+    @property
+    def weight(self):
+        return self.buffer[self.experts:].view(torch.float32)[:self.experts]
+
+    @property
+    def loss(self):
+        return self.buffer[self.experts:].view(torch.float32)[self.experts:self.experts + 1]
+
+
+@functools.lru_cache(maxsize=4096)
+def _balance_ws(T, E):
+    return int(fn('hetu_moe_balance_ws', [I64, I32], I64)(T, E))
 
 
 def _balance_operands(name, logits, valid):
@@ -160,27 +179,25 @@ def balance_loss(logits, indices, num_experts, valid=None):
     if native(x):
         check_device(x, 'balance_loss')
         idx = _dc(idx)
-        loss = _NA.empty((1,), dtype=torch.float32, device=x.device)
-        counts = _NA.empty((E,), dtype=torch.int64, device=x.device)
-        weight = _NA.empty((E,), dtype=torch.float32, device=x.device)
-        nws = int(fn('hetu_moe_balance_ws', [I64, I32], I64)(T, E))
-        ws = _NA.empty((nws,), dtype=torch.int32, device=x.device) if nws else None
-        f = fn('hetu_moe_balance_fwd', [P, I64, I64, I32, P, I32, P, I32, P, P, P, P, I32, P])
+        r = BalanceLoss(_NA.empty((E + E // 2 + 1,), dtype=torch.int64, device=x.device), E)
+        ws = _NA.empty((_balance_ws(T, E),), dtype=torch.int32, device=x.device)
+        f = fn('hetu_moe_balance_fwd', [P, I64, I64, I32, P, I32, P, I32, P, P, I32, P])
         check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, idx.data_ptr(), max(k, 1), ptr_or_none(valid),
-                _VALID_KINDS[valid.dtype] if valid is not None else 0, counts.data_ptr(), weight.data_ptr(),
-                loss.data_ptr(), ptr_or_none(ws), is_bf16(x), stream_ptr()), 'moe_balance')
+                _VALID_KINDS[valid.dtype] if valid is not None else 0, r.buffer.data_ptr(), ws.data_ptr(), is_bf16(x),
+                stream_ptr()), 'moe_balance')
         record_native('moe_balance')
-        return BalanceLoss(loss, counts, weight)
+        return r
+    r = BalanceLoss(torch.zeros(E + E // 2 + 1, dtype=torch.int64, device=x.device), E)
     on = torch.ones(T, dtype=torch.bool, device=x.device) if valid is None else valid != 0
     chosen = idx[on].reshape(-1)
     chosen = chosen[(chosen >= 0) & (chosen < E)]
-    counts = torch.bincount(chosen, minlength=E)
+    r.counts.copy_(torch.bincount(chosen, minlength=E))
     n = int(on.sum())
-    if n == 0:
-        return BalanceLoss(_NA.zeros(1, device=x.device), counts, _NA.zeros(E, device=x.device))
-    weight = E * counts.double() / (float(n) * n)
-    loss = (weight * torch.softmax(x[on].float(), 1).double().sum(0)).sum().reshape(1)
-    return BalanceLoss(loss.float(), counts, weight.float())
+    if n:
+        weight = E * r.counts.double() / (float(n) * n)
+        r.weight.copy_(weight)
+        r.loss.copy_((weight * torch.softmax(x[on].float(), 1).double().sum(0)).sum())
+    return r
 
 
 def balance_loss_backward(logits, fwd, grad, valid=None):
@@ -188,16 +205,16 @@ def balance_loss_backward(logits, fwd, grad, valid=None):
     fp32 value); ``fwd`` is what ``balance_loss`` gave for the same logits and ``valid``.  Tokens
     that are not valid get 0."""
     x, valid, T, E = _balance_operands('balance_loss_backward', logits, valid)
-    if fwd.weight.numel() != E or grad.numel() != 1 or grad.device != x.device:
+    if fwd.experts != E or grad.numel() != 1 or grad.device != x.device:
         raise ValueError('balance_loss_backward: %d experts, weights of %d, a gradient of %s'
-                         % (E, fwd.weight.numel(), tuple(grad.shape)))
+                         % (E, fwd.experts, tuple(grad.shape)))
     if native(x):
         check_device(x, 'balance_loss_backward')
         grad = _dc(grad, torch.float32)
         dx = _NA.empty((T, E), dtype=x.dtype, device=x.device)
         f = fn('hetu_moe_balance_bwd', [P, I64, I64, I32, P, P, P, I32, P, I32, P])
-        check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, fwd.weight.data_ptr(), grad.data_ptr(),
-                ptr_or_none(valid), _VALID_KINDS[valid.dtype] if valid is not None else 0, dx.data_ptr(), is_bf16(x),
+        check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, fwd.buffer.data_ptr() + 8 * E,
+                grad.data_ptr(), ptr_or_none(valid), _VALID_KINDS[valid.dtype] if valid is not None else 0, dx.data_ptr(), is_bf16(x),
                 stream_ptr()), 'moe_balance_bwd')
         record_native('moe_balance_bwd')
         return dx

@@ -247,6 +247,7 @@ def _shape(size):
 
 
 _BFC = [None]
+_POOL = [None]        # the memory_pool module (an import statement costs a call into importlib)
 _CPU = torch.device('cpu')
 
 
@@ -256,8 +257,10 @@ def _device_ok(device):
     if device.type != 'cuda':
         return True
     if _BFC[0] is None:
-        from . import memory_pool
-        if not memory_pool.torch_bfc_enabled():
+        if _POOL[0] is None:
+            from . import memory_pool
+            _POOL[0] = memory_pool
+        if not _POOL[0].torch_bfc_enabled():
             return False      # (not cached: the pool may still be installed later)
         _BFC[0] = True
     return _BFC[0]
