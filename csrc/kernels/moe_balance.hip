@@ -110,17 +110,18 @@ __device__ __forceinline__ void rows_exp(int E, int lane, float (&p)[U][NJ * V],
   for (int u = 0; u < U; ++u) inv[u] = __builtin_amdgcn_rcpf(group_sum(inv[u], G));
 }
 
-// Partial sums of block b: psum [b][E], counts [b][E + 1] (the last: valid tokens).  A group takes
+// Partial sums of block b, a row of 2 pitch + 4 words: E sums, E counts, the valid tokens, each part
+// starting 16-byte aligned.  A group takes
 // U rows at a time: the next U rows' loads and the validity of those after them are under way
 // while these are summed.
+__host__ __device__ inline int part_pitch(int E) { return (E + 3) & ~3; }
 constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;
 
 template <typename T, int V, int NJ, int G>
 __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restrict__ x, int64_t stride, int64_t T_,
                                                                int E, const int64_t* __restrict__ idx, int k,
                                                                const void* valid, int kind, int64_t rows,
-                                                               float* __restrict__ psum, int* __restrict__ pcnt,
-                                                               unsigned* __restrict__ ticket) {
+                                                               float* __restrict__ parts, unsigned* __restrict__ ticket) {
   constexpr int N = NJ * V, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1), CU = 4, groups = kPartThreads / G;
   constexpr int64_t step = groups * U;
   extern __shared__ int lds[];
@@ -209,80 +210,92 @@ __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restri
     }
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kPartThreads) {
+  const int pitch = part_pitch(E);
+  float* sums = parts + (int64_t)blockIdx.x * (2 * pitch + 4);
+  int* cnts = reinterpret_cast<int*>(sums) + pitch;
+  for (int e = tid; e < pitch; e += kPartThreads) {
     float s = 0.f;
+    if (e < E) {
 #pragma unroll
-    for (int w = 0; w < kPartWaves; ++w) s += cols[w * E + e];
-    psum[(int64_t)blockIdx.x * E + e] = s;
+      for (int w = 0; w < kPartWaves; ++w) s += cols[w * E + e];
+    }
+    sums[e] = s;
+    cnts[e] = e < E ? hist[e] : 0;
   }
-  for (int e = tid; e <= E; e += kPartThreads) pcnt[(int64_t)blockIdx.x * (E + 1) + e] = hist[e];
+  if (tid == 0) cnts[pitch] = hist[E];
 }
 
-// Counts, the weights of the backward pass and the loss from the blocks' sums: EB experts a
-// block, the partial sums of one expert over 1024 / EB threads, all in a fixed order.  The block
-// that comes last adds up the blocks' parts of the loss, in order too.
-constexpr int kJoinThreads = 1024, kJoinExperts = 16;
+// Counts, the weights of the backward pass and the loss from the blocks' sums: 16 experts a block,
+// 4 a thread and the blocks' rows over 256 threads, joined in a fixed order.  The block that
+// comes last adds up the blocks' parts of the loss, in order too.
+constexpr int kJoinThreads = 1024, kJoinExperts = 16, kJoinWaves = kJoinThreads / 64;
 
-__global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __restrict__ psum,
-                                                               const int* __restrict__ pcnt, int blocks, int E, int EB,
+__global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __restrict__ parts, int blocks, int E,
                                                                int64_t* __restrict__ counts, float* __restrict__ weight,
-                                                               float* __restrict__ loss, double* part, unsigned* ticket) {
-  __shared__ double sums[kJoinThreads];
-  __shared__ int64_t cnts[kJoinThreads];
-  __shared__ int64_t wave_n[kJoinThreads / 64];
-  __shared__ bool last;
-  const int tid = threadIdx.x, e = blockIdx.x * EB + (tid & (EB - 1)), seg = tid / EB, segs = kJoinThreads / EB;
+                                                               float* __restrict__ loss, double* loss_part,
+                                                               unsigned* ticket) {
+  __shared__ double sums[kJoinWaves][kJoinExperts];
+  __shared__ int64_t cnts[kJoinWaves][kJoinExperts], valid[kJoinWaves][4];
+  const int tid = threadIdx.x, pitch = part_pitch(E), words = 2 * pitch + 4;
+  const int e0 = blockIdx.x * kJoinExperts + (tid & 3) * 4, seg = tid >> 2;
   int64_t n = 0;
-  for (int b = tid; b < blocks; b += kJoinThreads) n += pcnt[(int64_t)b * (E + 1) + E];
+  for (int b = tid; b < blocks; b += kJoinThreads)
+    n += reinterpret_cast<const int*>(parts)[(int64_t)b * words + 2 * pitch];
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  int64_t c[4] = {0, 0, 0, 0};
+  if (e0 < E) {
+#pragma unroll 4
+    for (int b = seg; b < blocks; b += kJoinThreads / 4) {
+      const float* p = parts + (int64_t)b * words + e0;
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      const int4 w = *reinterpret_cast<const int4*>(p + pitch);
+      s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+      c[0] += w.x; c[1] += w.y; c[2] += w.z; c[3] += w.w;
+    }
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  if ((tid & 63) == 0) wave_n[tid >> 6] = n;
-  double s = 0.0;
-  int64_t c = 0;
+  for (int i = 0; i < 4; ++i) {
+    s[i] = quad_place_sum(s[i]);
+    c[i] = quad_place_sum(c[i]);
+  }
+  n = quad_place_sum(n);
+  if ((tid & 63) < 4) {
+    valid[tid >> 6][tid & 3] = n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sums[tid >> 6][(tid & 3) * 4 + i] = s[i];
+      cnts[tid >> 6][(tid & 3) * 4 + i] = c[i];
+    }
+  }
+  __syncthreads();
+  if (tid >= kJoinExperts) return;
+  double l = 0.0;
+  int64_t total = 0, count = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinWaves; ++w) {
+    l += sums[w][tid];
+    count += cnts[w][tid];
+    total += (valid[w][0] + valid[w][1]) + (valid[w][2] + valid[w][3]);
+  }
+  const int e = blockIdx.x * kJoinExperts + tid;
+  const double d = (double)total, w = total > 0 ? (double)E * (double)count / (d * d) : 0.0;
+  l = total > 0 && e < E ? w * l : 0.0;
   if (e < E) {
-#pragma unroll 8
-    for (int b = seg; b < blocks; b += segs) {
-      s += psum[(int64_t)b * E + e];
-      c += pcnt[(int64_t)b * (E + 1) + e];
-    }
+    counts[e] = count;
+    weight[e] = (float)w;
   }
-  sums[tid] = s;
-  cnts[tid] = c;
-  __syncthreads();
-  int64_t total = 0;
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 64; ++i) total += wave_n[i];
-  for (int h = segs >> 1; h > 0; h >>= 1) {
-    if (seg < h) {
-      sums[tid] += sums[tid + h * EB];
-      cnts[tid] += cnts[tid + h * EB];
-    }
-    __syncthreads();
-  }
-  if (tid < EB) {
-    double l = 0.0;
-    if (e < E) {
-      const double d = (double)total, w = total > 0 ? (double)E * (double)cnts[tid] / (d * d) : 0.0;
-      counts[e] = cnts[tid];
-      weight[e] = (float)w;
-      l = total > 0 ? w * sums[tid] : 0.0;
-    }
-    sums[tid] = l;
-  }
-  __syncthreads();
-  if (tid < 64) {
-    double l = tid < EB ? sums[tid] : 0.0;
-#pragma unroll
-    for (int o = kJoinExperts / 2; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-    sums[tid] = l;
-  }
+  for (int o = 1; o < kJoinExperts; o <<= 1) l += __shfl_xor(l, o, 64);
   if (tid == 0) {
-    double l = sums[0];
-    __hip_atomic_store(part + blockIdx.x, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-    if (last) {
+    if (gridDim.x == 1) {
+      loss[0] = (float)l;
+      return;
+    }
+    __hip_atomic_store(loss_part + blockIdx.x, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
       l = 0.0;
-      for (unsigned i = 0; i < gridDim.x; ++i) l += __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (unsigned i = 0; i < gridDim.x; ++i)
+        l += __hip_atomic_load(loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       loss[0] = (float)l;
     }
   }
@@ -409,14 +422,14 @@ static void with_plan(const RowPlan& r, F f) {
   }
 }
 
-// number of 4-byte words of workspace (8-byte aligned) that hetu_moe_balance_fwd needs: each
-// block's sums and counts, the joining blocks' parts of the loss, their ticket
+// number of 4-byte words of workspace (16-byte aligned) that hetu_moe_balance_fwd needs: the
+// joining blocks' parts of the loss, their ticket, each block's sums and counts
 HETU_API int64_t hetu_moe_balance_ws(int64_t T, int E) {
   if (T < 0 || E < 1 || E > kMaxExperts) return 0;
   const int64_t groups_least = kPartThreads / 64;
   int64_t parts = (T + groups_least * 8 - 1) / (groups_least * 8);
   parts = parts < 1 ? 1 : (parts > kMaxParts ? kMaxParts : parts);
-  return 2 * (kMaxExperts / kJoinExperts) + 2 + parts * (2 * E + 1);
+  return 2 * (kMaxExperts / kJoinExperts) + 4 + parts * (2 * part_pitch(E) + 4);
 }
 
 // counts: a buffer of E int64, then (as fp32) E weights and the loss
@@ -430,22 +443,18 @@ HETU_API int hetu_moe_balance_fwd(const void* x, int64_t stride, int64_t T, int 
   float *weight = (float*)(counts + E), *loss = weight + E;
   double* part = (double*)ws;
   unsigned* ticket = (unsigned*)(part + kMaxExperts / kJoinExperts);
-  float* psum = (float*)(ticket + 2);
-  int* pcnt = (int*)(psum + (int64_t)blocks * E);
+  float* sums = (float*)(ticket + 4);
   const size_t lds = sizeof(int) * (size_t)(E + 1 + kPartWaves * E);
   const auto go = [&](auto zero, auto v, auto nj, auto g) {
     typedef decltype(zero) TT;
     hipLaunchKernelGGL((balance_part_k<TT, decltype(v)::value, decltype(nj)::value, decltype(g)::value>), dim3(blocks),
-                       dim3(kPartThreads), lds, st, (const TT*)x, stride, T, E, idx, k, valid, kind, rows, psum, pcnt,
-                       ticket);
+                       dim3(kPartThreads), lds, st, (const TT*)x, stride, T, E, idx, k, valid, kind, rows, sums, ticket);
   };
   if (is_bf16) with_plan<8>(r, [&](auto v, auto nj, auto g) { go(bf16(), v, nj, g); });
   else with_plan<4>(r, [&](auto v, auto nj, auto g) { go(0.f, v, nj, g); });
   HETU_LAUNCH_CHECK();
-  int EB = 1;
-  while (EB < E && EB < kJoinExperts) EB <<= 1;
-  hipLaunchKernelGGL(balance_join_k, dim3((E + EB - 1) / EB), dim3(kJoinThreads), 0, st, psum, pcnt, blocks, E, EB,
-                     counts, weight, loss, part, ticket);
+  hipLaunchKernelGGL(balance_join_k, dim3((E + kJoinExperts - 1) / kJoinExperts), dim3(kJoinThreads), 0, st, sums,
+                     blocks, E, counts, weight, loss, part, ticket);
   HETU_LAUNCH_CHECK();
   return 0;
 }

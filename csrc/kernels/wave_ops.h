@@ -54,4 +54,33 @@ __device__ __forceinline__ float group_sum(float v, int G) {
   }));
 }
 
+// sum over the lanes with the same place in their quad (16 of a wave), of a 64-bit number or double
+template <typename T>
+__device__ __forceinline__ T quad_place_sum(T v) {
+  static_assert(sizeof(T) == 8, "two words");
+  const auto pair = [](unsigned lo, unsigned hi) {
+    const uint64_t b = ((uint64_t)hi << 32) | lo;
+    T r;
+    __builtin_memcpy(&r, &b, 8);
+    return r;
+  };
+  const auto words = [](T x) {
+    uint64_t b;
+    __builtin_memcpy(&b, &x, 8);
+    return b;
+  };
+  uint64_t b = words(v);
+  v += pair(dpp<0x128>((unsigned)b), dpp<0x128>((unsigned)(b >> 32)));      // row_ror:8
+  b = words(v);
+  v += pair(dpp<0x124>((unsigned)b), dpp<0x124>((unsigned)(b >> 32)));      // row_ror:4
+  b = words(v);
+  const auto l = __builtin_amdgcn_permlane16_swap((unsigned)b, (unsigned)b, false, false);
+  const auto h = __builtin_amdgcn_permlane16_swap((unsigned)(b >> 32), (unsigned)(b >> 32), false, false);
+  v = pair(l[0], h[0]) + pair(l[1], h[1]);
+  b = words(v);
+  const auto l2 = __builtin_amdgcn_permlane32_swap((unsigned)b, (unsigned)b, false, false);
+  const auto h2 = __builtin_amdgcn_permlane32_swap((unsigned)(b >> 32), (unsigned)(b >> 32), false, false);
+  return pair(l2[0], h2[0]) + pair(l2[1], h2[1]);
+}
+
 }  // namespace hetu
