@@ -18,7 +18,7 @@
 //     57344: rounding up cannot overflow.
 // NaN and Inf in a gradient stay with their elements (the e4m3 NaN, the e5m2 Inf or NaN), as with
 // 32-bit moments: the scale is taken over the finite elements of the block.
-#include "common.h"
+#include "wave_ops.h"
 
 namespace hetu {
 
@@ -32,40 +32,48 @@ struct Adam8Args {
   uint64_t seed;
 };
 
-constexpr int kBlock8 = 256;   // elements that share a scale: 4 a lane, one wave
+constexpr int kBlock8 = 256;   // elements that share a scale: 8 a lane, half a wave
+constexpr int kLane8 = 8;
 
-// a 32-bit mix (multiply, xor-shift) of the element's index and the step's seed: the low half
-// rounds m, the high half v
-__device__ __forceinline__ unsigned round_bits(unsigned idx, unsigned seed) {
-  unsigned h = idx * 0x9E3779B1u + seed;
+// a 32-bit mix (multiply, xor-shift) of a number made from the element's index and the step's
+// seed: the low half rounds m, the high half v
+__device__ __forceinline__ unsigned round_bits(unsigned h) {
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;
   return h ^ (h >> 16);
 }
 
-// |y| (finite, below the format's largest power of two) as a code of MANT mantissa bits, exponent
-// bias BIAS: r16 is added below the last bit kept (half a unit of r16 on top, so that 16 bits
-// round without bias), in the mantissa of a normal, in fixed point where the code is a subnormal
-template <int MANT, int BIAS>
-__device__ __forceinline__ unsigned encode8(float y, unsigned r16) {
-  constexpr int CUT = 23 - MANT;
-  const unsigned r = (r16 << (CUT - 16)) | (1u << (CUT - 17));
-  const unsigned normal = ((__float_as_uint(y) + r) >> CUT) - ((127u - BIAS) << MANT);
-  const float least = __uint_as_float((unsigned)(128 - BIAS) << 23);            // 2^(1 - BIAS)
-  const float units = __uint_as_float((unsigned)(127 + BIAS + 22) << 23);       // 2^(BIAS + 22)
-  const unsigned small = ((unsigned)(int)(y * units) + r) >> CUT;
-  return y < least ? small : normal;
+// Codes in the top byte of a word (a sign bit of 0).  The value is scaled so that the format's
+// smallest normal number becomes fp32's: its bits then are the code's, the subnormals' too, with
+// the rest of the mantissa below.  To these the 16 random bits are added, aligned with the highest
+// bit cut off, and half a unit of them, so that 16 bits round without bias.
+//   e4m3 (bias 7): x 2^(7 - se), the code from bit 20 up;  e5m2 (bias 15): x 2^(15 - se), bit 21
+// where 2^(se - 127) is the block's scale.
+__device__ __forceinline__ unsigned encode_m(float m, int se, unsigned h) {
+  const unsigned bits = __float_as_uint(__builtin_amdgcn_ldexpf(fabsf(m), 7 - se));
+  const unsigned t = (bits + (((h << 4) & 0xFFFF0u) | 8u)) << 4;
+  return t | (__float_as_uint(m) & 0x80000000u);
+}
+__device__ __forceinline__ unsigned encode_v(float v, int se, unsigned h) {
+  const unsigned bits = __float_as_uint(__builtin_amdgcn_ldexpf(v, 15 - se));
+  const unsigned t = (bits + (((h >> 11) & 0x1FFFE0u) | 16u)) << 3;
+  const unsigned least = v > 0.f ? 1u << 24 : 0u;
+  return t > least ? t : least;
 }
 
-__device__ __forceinline__ float decode_m(unsigned c) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
-}
-__device__ __forceinline__ float decode_v(unsigned c) {
-  return __builtin_amdgcn_cvt_f32_bf8((int)c, 0);
+// the top bytes of four words as one
+__device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0C0C0703u), hi = __builtin_amdgcn_perm(d, c, 0x07030C0Cu);
+  return lo | hi;
 }
 
-// One wave a block of 256 elements, 4 a lane: the block's largest exponents are one reduction
-// over the wave.  VEC: every buffer lets a lane move its 4 elements at once.
+// Half a wave a block of 256 elements, 8 a lane: the block's largest exponents are five lane
+// exchanges.  VEC: every buffer lets a lane move its elements in 16 and 8 bytes at once.
+//
+// What bounds it: 16 bytes an element to move (18 with the copy), and about 60 issue slots of the
+// vector unit, where 128 would take as long as the memory.  So no division and no exact root in
+// the update, where a unit of fp32 does not matter (v_rcp_f32, v_sqrt_f32: 1 unit each; the root
+// of a v below 2^-126 is 0, which an eps of 1e-12 or more does not feel).
 template <bool SHADOW, bool VEC>
 __global__ void __launch_bounds__(256) adamw8_k(float* __restrict__ p, const float* __restrict__ g,
                                                  unsigned char* __restrict__ mc, unsigned char* __restrict__ vc,
@@ -73,81 +81,111 @@ __global__ void __launch_bounds__(256) adamw8_k(float* __restrict__ p, const flo
                                                  unsigned short* __restrict__ shadow, int64_t n, int64_t nb,
                                                  Adam8Args a) {
 #pragma clang fp contract(off)   // the moments are rounded operation by operation, as documented
-  const int lane = threadIdx.x & 63;
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * 4;
+  constexpr int N = kLane8;
+  const int lane = threadIdx.x & 31;
+  const int64_t half = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), halves = (int64_t)gridDim.x * 8;
   float lr = a.lr, c1 = a.omb1t, c2 = a.omb2t, gsc = a.gscale;
   uint64_t key = a.seed;
   if (a.dyn) {
     lr = a.dyn[0]; gsc = a.dyn[3]; c1 = a.dyn[5]; c2 = a.dyn[6];
     key += (uint64_t)a.dyn[4] * kRngMix;
   }
+  const float r1 = 1.f / c1, r2 = 1.f / c2;
   const unsigned seed = (unsigned)key ^ (unsigned)(key >> 32);
-  for (int64_t b = wave; b < nb; b += waves) {
-    const int64_t i0 = b * kBlock8 + lane * 4;
-    const int cnt = n - i0 >= 4 ? 4 : (n > i0 ? (int)(n - i0) : 0);
-    float pv[4] = {0, 0, 0, 0}, gv[4] = {0, 0, 0, 0}, m[4], v[4];
-    unsigned mq = 0, vq = 0;
-    if (VEC && cnt == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(p + i0), y = *reinterpret_cast<const float4*>(g + i0);
-      pv[0] = x.x; pv[1] = x.y; pv[2] = x.z; pv[3] = x.w;
-      gv[0] = y.x; gv[1] = y.y; gv[2] = y.z; gv[3] = y.w;
-      mq = *reinterpret_cast<const unsigned*>(mc + i0);
-      vq = *reinterpret_cast<const unsigned*>(vc + i0);
+  for (int64_t b = half; b < nb; b += halves) {
+    const int64_t i0 = b * kBlock8 + lane * N;
+    const int cnt = n - i0 >= N ? N : (n > i0 ? (int)(n - i0) : 0);
+    float pv[N], gv[N], m[N], v[N];
+    unsigned mq[2] = {0, 0}, vq[2] = {0, 0};
+    if (VEC && cnt == N) {
+      load_vec<float>(p + i0, reinterpret_cast<float(&)[4]>(pv[0]));
+      load_vec<float>(p + i0 + 4, reinterpret_cast<float(&)[4]>(pv[4]));
+      load_vec<float>(g + i0, reinterpret_cast<float(&)[4]>(gv[0]));
+      load_vec<float>(g + i0 + 4, reinterpret_cast<float(&)[4]>(gv[4]));
+      const uint2 x = *reinterpret_cast<const uint2*>(mc + i0), y = *reinterpret_cast<const uint2*>(vc + i0);
+      mq[0] = x.x; mq[1] = x.y;
+      vq[0] = y.x; vq[1] = y.y;
     } else {
-      for (int k = 0; k < cnt; ++k) {
-        pv[k] = p[i0 + k];
-        gv[k] = g[i0 + k];
-        mq |= (unsigned)mc[i0 + k] << (8 * k);
-        vq |= (unsigned)vc[i0 + k] << (8 * k);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        pv[k] = k < cnt ? p[i0 + k] : 0.f;
+        gv[k] = k < cnt ? g[i0 + k] : 0.f;
+        mq[k >> 2] |= (unsigned)(k < cnt ? mc[i0 + k] : 0) << (8 * (k & 3));
+        vq[k >> 2] |= (unsigned)(k < cnt ? vc[i0 + k] : 0) << (8 * (k & 3));
       }
     }
-    const float msc = ms[b], vsc = vs[b];
-    float mtop = 0.f, vtop = 0.f;
+    // beta times the scale, a power of two: exact
+    const float bm = a.beta1 * ms[b], bv = a.beta2 * vs[b];
+    unsigned mtop = 0, vtop = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < N; ++k) {
+      const int w = k >> 2;
       const float gr = gv[k] * gsc;
-      m[k] = a.beta1 * (decode_m((mq >> (8 * k)) & 255u) * msc) + a.omb1 * gr;
-      v[k] = a.beta2 * (decode_v((vq >> (8 * k)) & 255u) * vsc) + a.omb2 * gr * gr;
-      const float u = (m[k] / c1) / (sqrtf(v[k] / c2) + a.eps);
-      pv[k] -= lr * (u + a.wd * pv[k]);
-      if (k >= cnt) m[k] = v[k] = 0.f;
-      const float am = fabsf(m[k]);
-      if (am < INFINITY) mtop = fmaxf(mtop, am);
-      if (v[k] < INFINITY) vtop = fmaxf(vtop, v[k]);
+      const auto dm = (k & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)mq[w], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)mq[w], false);
+      const auto dv = (k & 2) ? __builtin_amdgcn_cvt_pk_f32_bf8((int)vq[w], true) : __builtin_amdgcn_cvt_pk_f32_bf8((int)vq[w], false);
+      m[k] = dm[k & 1] * bm + a.omb1 * gr;
+      v[k] = dv[k & 1] * bv + a.omb2 * gr * gr;
+      const float root = __builtin_amdgcn_sqrtf(v[k] * r2) + a.eps;
+      const float u = m[k] * r1 * __builtin_amdgcn_rcpf(root);
+      pv[k] = __builtin_fmaf(-lr, __builtin_fmaf(a.wd, pv[k], u), pv[k]);
+      const unsigned am = __float_as_uint(m[k]) & 0x7FFFFFFFu, av = __float_as_uint(v[k]);
+      mtop = mtop > am ? mtop : am;
+      vtop = vtop > av ? vtop : av;
     }
-    mtop = wave_max(mtop);
-    vtop = wave_max(vtop);
-    // 2^(floor(log2(largest)) - 7), - 14, not below the smallest normal
-    int me = (int)(__float_as_uint(mtop) >> 23) - 7, ve = (int)(__float_as_uint(vtop) >> 23) - 14;
+    const auto larger = [](unsigned x, unsigned y) { return x > y ? x : y; };
+    mtop = group_join(mtop, 32, larger);
+    vtop = group_join(vtop, 32, larger);
+    const bool odd = mtop >= 0x7F800000u || vtop >= 0x7F800000u;
+    if (odd) {                     // an Inf or NaN in the block: the largest of the others
+      mtop = vtop = 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const unsigned am = __float_as_uint(m[k]) & 0x7FFFFFFFu, av = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+        if (am < 0x7F800000u) mtop = larger(mtop, am);
+        if (av < 0x7F800000u) vtop = larger(vtop, av);
+      }
+      mtop = group_join(mtop, 32, larger);
+      vtop = group_join(vtop, 32, larger);
+    }
+    // the scales 2^(floor(log2(largest)) - 7), - 14, not below the smallest normal number
+    int me = (int)(mtop >> 23) - 7, ve = (int)(vtop >> 23) - 14;
     me = me < 1 ? 1 : me;
     ve = ve < 1 ? 1 : ve;
-    const float minv = __uint_as_float((unsigned)(254 - me) << 23), vinv = __uint_as_float((unsigned)(254 - ve) << 23);
-    mq = vq = 0;
+    unsigned em[N], ev[N];
+    const unsigned h0 = (unsigned)i0 * 0x9E3779B1u + seed;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const unsigned r = round_bits((unsigned)(i0 + k), seed);
-      const float am = fabsf(m[k]);
-      unsigned cm = am < INFINITY ? encode8<3, 7>(am * minv, r & 0xFFFFu) : 0x7Fu;
-      unsigned cv = v[k] < INFINITY ? encode8<2, 15>(v[k] * vinv, r >> 16) : (v[k] != v[k] ? 0x7Fu : 0x7Cu);
-      if (m[k] < 0.f) cm |= 0x80u;
-      if (v[k] > 0.f && cv == 0u) cv = 1u;
-      mq |= cm << (8 * k);
-      vq |= cv << (8 * k);
+    for (int k = 0; k < N; ++k) {
+      const unsigned h = round_bits(h0 + (unsigned)k * 0x9E3779B1u);
+      em[k] = encode_m(m[k], me, h);
+      ev[k] = encode_v(v[k], ve, h);
     }
-    if (VEC && cnt == 4) {
-      *reinterpret_cast<float4*>(p + i0) = make_float4(pv[0], pv[1], pv[2], pv[3]);
-      *reinterpret_cast<unsigned*>(mc + i0) = mq;
-      *reinterpret_cast<unsigned*>(vc + i0) = vq;
-      if (SHADOW)
-        *reinterpret_cast<uint2*>(shadow + i0) =
-            make_uint2((unsigned)f_to_bf16_bits(pv[0]) | ((unsigned)f_to_bf16_bits(pv[1]) << 16),
-                       (unsigned)f_to_bf16_bits(pv[2]) | ((unsigned)f_to_bf16_bits(pv[3]) << 16));
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      mq[w] = top_bytes(em[4 * w], em[4 * w + 1], em[4 * w + 2], em[4 * w + 3]);
+      vq[w] = top_bytes(ev[4 * w], ev[4 * w + 1], ev[4 * w + 2], ev[4 * w + 3]);
+    }
+    if (VEC && cnt == N) {
+      store_vec<float>(p + i0, reinterpret_cast<const float(&)[4]>(pv[0]));
+      store_vec<float>(p + i0 + 4, reinterpret_cast<const float(&)[4]>(pv[4]));
+      *reinterpret_cast<uint2*>(mc + i0) = make_uint2(mq[0], mq[1]);
+      *reinterpret_cast<uint2*>(vc + i0) = make_uint2(vq[0], vq[1]);
+      if (SHADOW) store_vec<bf16>(reinterpret_cast<bf16*>(shadow) + i0, pv);
     } else {
-      for (int k = 0; k < cnt; ++k) {
-        p[i0 + k] = pv[k];
-        mc[i0 + k] = (unsigned char)(mq >> (8 * k));
-        vc[i0 + k] = (unsigned char)(vq >> (8 * k));
-        if (SHADOW) shadow[i0 + k] = f_to_bf16_bits(pv[k]);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (k < cnt) {
+          p[i0 + k] = pv[k];
+          mc[i0 + k] = (unsigned char)(em[k] >> 24);
+          vc[i0 + k] = (unsigned char)(ev[k] >> 24);
+          if (SHADOW) shadow[i0 + k] = f_to_bf16_bits(pv[k]);
+        }
+      }
+    }
+    if (odd) {                     // their codes, over what the arithmetic above made of them
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (k < cnt && !(fabsf(m[k]) < INFINITY)) mc[i0 + k] = 0x7F;
+        if (k < cnt && !(v[k] < INFINITY)) vc[i0 + k] = v[k] != v[k] ? 0x7F : 0x7C;
       }
     }
     if (lane == 0) {
@@ -167,10 +205,10 @@ HETU_API int hetu_adamw8(float* p, const float* g, void* m, void* v, float* ms, 
   if (n <= 0) return 0;
   const int64_t nb = (n + kBlock8 - 1) / kBlock8;
   const Adam8Args a = {lr, beta1, beta2, omb1, omb2, omb1t, omb2t, eps, wd, gscale, dyn, (uint64_t)seed};
-  const int64_t want = (nb + 3) / 4;
+  const int64_t want = (nb + 7) / 8;
   const dim3 grid((unsigned)(want < 2048 ? want : 2048));
-  const bool vec = (((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)m | (uintptr_t)v) & 3) == 0 &&
-                   ((uintptr_t)shadow & 7) == 0;
+  const bool vec = (((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)m | (uintptr_t)v) & 7) == 0 &&
+                   ((uintptr_t)shadow & 15) == 0;
 #define GO(S, V) hipLaunchKernelGGL((adamw8_k<S, V>), grid, dim3(256), 0, st, p, g, (unsigned char*)m, (unsigned char*)v, \
                                     ms, vs, (unsigned short*)shadow, n, nb, a)
   if (shadow) { if (vec) GO(true, true); else GO(true, false); }

@@ -128,13 +128,12 @@ def _round_bits(n, seed, device):
 
 
 def _encode8(y, r16, mant, bias):
-    """adamw8.hip ``encode8``"""
+    """adamw8.hip ``encode_m`` / ``encode_v``: codes of y = |x| / scale, whose bits once it is
+    multiplied by 2^(bias - 127) are the code's, with the part to be cut off below"""
     cut = 23 - mant
     r = ((r16 << (cut - 16)) | (1 << (cut - 17))).int()
-    y = torch.where(torch.isfinite(y), y, torch.zeros_like(y))
-    normal = ((y.view(torch.int32) + r) >> cut) - ((127 - bias) << mant)
-    small = ((y * 2.0 ** (bias + 22)).int() + r) >> cut
-    return torch.where(y < 2.0 ** (1 - bias), small, normal)
+    y = torch.where(torch.isfinite(y), y, torch.zeros_like(y)) * 2.0 ** (bias - 127)
+    return (y.view(torch.int32) + r) >> cut
 
 
 def _scale8(x, nb, top):
@@ -154,7 +153,7 @@ def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.
     instead of the arguments, for a captured step; the seed is then moved by ``step`` as
     ``step_seed`` moves it.
     ``shadow`` (bf16, the weights' copy) is written too.  A block of 256 shares one scale: where
-    several tensors share the buffer, start each at a multiple of 256."""
+    several tensors share the buffer, start each at a multiple of 256.  ``eps`` is at least 1e-12."""
     n = p.numel()
     nb = -(-n // STATE8_BLOCK)
     for t, dt, size, what in ((p, torch.float32, n, 'p'), (g, torch.float32, n, 'g'), (m, torch.float8_e4m3fn, n, 'm'),
@@ -166,6 +165,8 @@ def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.
         if t.dtype != dt or t.numel() != size or not t.is_contiguous() or t.device != p.device:
             raise ValueError('adamw8: %s has to be a contiguous %s of %d elements on %s, got %s %s on %s'
                              % (what, dt, size, p.device, t.dtype, tuple(t.shape), t.device))
+    if not eps >= 1e-12:
+        raise ValueError('adamw8: eps has to be at least 1e-12, got %r' % (eps,))
     if n == 0:
         return
     if native(p):

@@ -196,6 +196,9 @@ def test_refusals():
         KO.adamw8(*s, torch.zeros(300), **H)
     with pytest.raises(ValueError):
         KO.adamw8(*s, dyn=torch.zeros(4), **H)
+    for eps in (0.0, 1e-13, float('nan')):
+        with pytest.raises(ValueError):
+            KO.adamw8(*s, **dict(H, eps=eps))
     with pytest.raises(ValueError):
         ht.optim.AdamWOptimizer(state_bits=4)
     KO.adamw8(*[t[:0] for t in s], **H)                     # no elements: nothing to do
