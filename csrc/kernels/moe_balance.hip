@@ -67,6 +67,13 @@ struct RowRaw {
       else q[j] = *reinterpret_cast<const Q4*>(x + e);
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if constexpr (V == 1) s[j] = from_f<T>(0.f);
+      else q[j] = Q4{0, 0, 0, 0};
+    }
+  }
   __device__ __forceinline__ void unpack(float (&p)[NJ * V]) const {
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -111,7 +118,7 @@ __device__ __forceinline__ void rows_exp(int E, int lane, float (&p)[U][NJ * V],
 }
 
 // Partial sums of block b, a row of 2 pitch + 4 words: E sums, E counts, the valid tokens, each part
-// starting 16-byte aligned.  A group takes
+// starting 16-byte aligned; of a single block the results (counts: hetu_moe_balance_fwd).  A group takes
 // U rows at a time: the next U rows' loads and the validity of those after them are under way
 // while these are summed.
 __host__ __device__ inline int part_pitch(int E) { return (E + 3) & ~3; }
@@ -121,10 +128,11 @@ template <typename T, int V, int NJ, int G>
 __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restrict__ x, int64_t stride, int64_t T_,
                                                                int E, const int64_t* __restrict__ idx, int k,
                                                                const void* valid, int kind, int64_t rows,
-                                                               float* __restrict__ parts, unsigned* __restrict__ ticket) {
-  constexpr int N = NJ * V, U = N <= 8 ? 4 : (N <= 16 ? 2 : 1), CU = 4, groups = kPartThreads / G;
+                                                               float* __restrict__ parts, unsigned* __restrict__ ticket,
+                                                               int64_t* __restrict__ counts) {
+  constexpr int N = NJ * V, U = N <= 8 ? 4 : 1, CU = 4, groups = kPartThreads / G;
   constexpr int64_t step = groups * U;
-  extern __shared__ int lds[];
+  extern __shared__ __align__(16) int lds[];
   int* hist = lds;                                       // [E + 1]
   float* cols = reinterpret_cast<float*>(lds + E + 1);   // [kPartWaves][E]
   const int tid = threadIdx.x, lane = tid & (G - 1), group = tid / G;
@@ -177,6 +185,7 @@ __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restri
     bool now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (!on[u]) raw[u].clear();
       raw[u].unpack(p[u]);
       now[u] = on[u];
       on[u] = next[u];
@@ -189,16 +198,16 @@ __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restri
     rows_exp<U, V, NJ, G>(E, lane, p, inv);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const float c = now[u] ? inv[u] : 0.f;          // (a row in another's place is finite: zeroed)
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += now[u] ? p[u][i] * inv[u] : 0.f;
+      for (int i = 0; i < N; ++i) acc[i] += p[u][i] * c;
       count += now[u];
     }
   }
   if (lane == 0 && count) atomicAdd(&hist[E], count);
   // groups of a wave, then waves
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    for (int o = G; o < 64; o <<= 1) acc[i] += __shfl_xor(acc[i], o, 64);
+  for (int i = 0; i < N; ++i) acc[i] = place_sum<G>(acc[i]);
   if ((tid & 63) < G) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -210,6 +219,30 @@ __global__ void __launch_bounds__(kPartThreads) balance_part_k(const T* __restri
     }
   }
   __syncthreads();
+  if (gridDim.x == 1) {                // nothing to join: the results themselves
+    const double n = (double)hist[E];
+    double l = 0.0;
+    for (int e = tid; e < E; e += kPartThreads) {
+      double s = 0.0;
+#pragma unroll
+      for (int w = 0; w < kPartWaves; ++w) s += cols[w * E + e];
+      const double c = n > 0.0 ? (double)E * hist[e] / (n * n) : 0.0;
+      counts[e] = hist[e];
+      reinterpret_cast<float*>(counts + E)[e] = (float)c;
+      l += c * s;
+    }
+    l = quad_place_sum(l);
+    __syncthreads();                   // (cols are read: their place holds the waves' parts now)
+    double* part = reinterpret_cast<double*>(lds);
+    if ((tid & 63) < 4) part[(tid >> 6) * 4 + (tid & 3)] = l;
+    __syncthreads();
+    if (tid == 0) {
+      l = 0.0;
+      for (int i = 0; i < kPartWaves * 4; ++i) l += part[i];
+      reinterpret_cast<float*>(counts + E)[E] = (float)l;
+    }
+    return;
+  }
   const int pitch = part_pitch(E);
   float* sums = parts + (int64_t)blockIdx.x * (2 * pitch + 4);
   int* cnts = reinterpret_cast<int*>(sums) + pitch;
@@ -363,16 +396,17 @@ __global__ void __launch_bounds__(kBlThreads) balance_bwd_k(const T* __restrict_
 
 struct RowPlan { int V, G, NJ; };
 
-// V elements a load where rows and buffers allow 16-byte accesses, G lanes a row, NJ loads a lane
+// V elements a load where rows and buffers allow 16-byte accesses, G lanes a row, NJ loads a lane.
+// The vector unit bounds these kernels (about 9 issue slots an element, 5 more for each exchange of
+// a reduction and 15 for a row, in every lane), so a lane takes up to 16 elements and G is what they
+// leave: 262144 x 256 bf16 with 16 lanes a row against 32: see the measurements at the launches.
 static RowPlan plan_rows(int E, int64_t stride, const void* x, const void* y, int vec) {
   RowPlan r;
   r.V = (E % vec == 0 && stride % vec == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0) ? vec : 1;
-  const int units = (E + r.V - 1) / r.V;
   r.G = 1;
-  while (r.G < units && r.G < 64) r.G <<= 1;
-  const int nj = (units + r.G - 1) / r.G;
-  r.NJ = 1;
-  while (r.NJ < nj) r.NJ <<= 1;
+  while (16 * r.G < E) r.G <<= 1;
+  r.NJ = (E + r.V * r.G - 1) / (r.V * r.G);
+  if (r.V == 1) r.NJ = r.NJ <= 2 ? 2 : r.NJ <= 4 ? 4 : r.NJ <= 8 ? 8 : r.NJ <= 12 ? 12 : 16;
   return r;
 }
 
@@ -380,45 +414,48 @@ static RowPlan plan_rows(int E, int64_t stride, const void* x, const void* y, in
 
 using namespace hetu;
 
-// Rows a block of the partial sums takes: as many blocks as keep the chip's waves busy (4 blocks of 8
-// waves a CU), but at least 8 rows a group of lanes, for each block costs E partial sums.
-constexpr int kMaxParts = 1024;
+// Rows a block of the partial sums takes: as many blocks as keep the chip's waves busy (2 blocks of 8
+// waves a CU; 1024 blocks gain the partial sums nothing and cost the join 2 us), but at least 2 rows a group of lanes, for each block costs E partial sums.
+constexpr int kMaxParts = 512;
 static int64_t balance_rows(int64_t T, int G) {
   const int64_t groups = kPartThreads / G;
-  int64_t blocks = (T + groups * 8 - 1) / (groups * 8);
+  int64_t blocks = (T + groups * 2 - 1) / (groups * 2);
+  // one block has no join: that is worth up to 4 rows a group (96 x 8: 4.5 us for both launches' 8)
+  if (T <= groups * 4) blocks = 1;
   blocks = blocks < 1 ? 1 : (blocks > kMaxParts ? kMaxParts : blocks);
   return (T + blocks - 1) / blocks;
 }
 
-// calls f(V, NJ, G) as compile-time numbers for the plan
+// calls f(V, NJ, G) as compile-time numbers for the plan: more than one lane a row have 9 to 16
+// elements each
 template <int N> struct Const { static constexpr int value = N; };
 template <int V, int NJ, typename F>
 static void with_group(int G, F f) {
-  if constexpr (NJ > 1) f(Const<V>(), Const<NJ>(), Const<64>());
-  else if (G == 1) f(Const<V>(), Const<1>(), Const<1>());
-  else if (G == 2) f(Const<V>(), Const<1>(), Const<2>());
-  else if (G == 4) f(Const<V>(), Const<1>(), Const<4>());
-  else if (G == 8) f(Const<V>(), Const<1>(), Const<8>());
-  else if (G == 16) f(Const<V>(), Const<1>(), Const<16>());
-  else if (G == 32) f(Const<V>(), Const<1>(), Const<32>());
-  else f(Const<V>(), Const<1>(), Const<64>());
+  if (G == 1) f(Const<V>(), Const<NJ>(), Const<1>());
+  if constexpr (V * NJ > 8) {
+    if (G == 2) f(Const<V>(), Const<NJ>(), Const<2>());
+    if (G == 4) f(Const<V>(), Const<NJ>(), Const<4>());
+    if (G == 8) f(Const<V>(), Const<NJ>(), Const<8>());
+    if (G == 16) f(Const<V>(), Const<NJ>(), Const<16>());
+    if (G == 32) f(Const<V>(), Const<NJ>(), Const<32>());
+    if (G == 64) f(Const<V>(), Const<NJ>(), Const<64>());
+  }
 }
 template <int VEC, typename F>      // VEC: elements of 16 bytes
 static void with_plan(const RowPlan& r, F f) {
   if (r.V == VEC) {
     if (r.NJ == 1) with_group<VEC, 1>(r.G, f);
-    else if (r.NJ == 2) with_group<VEC, 2>(r.G, f);
-    else if constexpr (VEC == 4) with_group<VEC, 4>(r.G, f);
-  } else if (r.NJ == 1) {
-    with_group<1, 1>(r.G, f);
-  } else if (r.NJ == 2) {
-    with_group<1, 2>(r.G, f);
-  } else if (r.NJ == 4) {
-    with_group<1, 4>(r.G, f);
-  } else if (r.NJ == 8) {
-    with_group<1, 8>(r.G, f);
+    if (r.NJ == 2) with_group<VEC, 2>(r.G, f);
+    if constexpr (VEC == 4) {
+      if (r.NJ == 3) with_group<VEC, 3>(r.G, f);
+      if (r.NJ == 4) with_group<VEC, 4>(r.G, f);
+    }
   } else {
-    with_group<1, 16>(r.G, f);
+    if (r.NJ == 2) with_group<1, 2>(r.G, f);
+    if (r.NJ == 4) with_group<1, 4>(r.G, f);
+    if (r.NJ == 8) with_group<1, 8>(r.G, f);
+    if (r.NJ == 12) with_group<1, 12>(r.G, f);
+    if (r.NJ == 16) with_group<1, 16>(r.G, f);
   }
 }
 
@@ -427,7 +464,7 @@ static void with_plan(const RowPlan& r, F f) {
 HETU_API int64_t hetu_moe_balance_ws(int64_t T, int E) {
   if (T < 0 || E < 1 || E > kMaxExperts) return 0;
   const int64_t groups_least = kPartThreads / 64;
-  int64_t parts = (T + groups_least * 8 - 1) / (groups_least * 8);
+  int64_t parts = (T + groups_least * 2 - 1) / (groups_least * 2);
   parts = parts < 1 ? 1 : (parts > kMaxParts ? kMaxParts : parts);
   return 2 * (kMaxExperts / kJoinExperts) + 4 + parts * (2 * part_pitch(E) + 4);
 }
@@ -444,16 +481,18 @@ HETU_API int hetu_moe_balance_fwd(const void* x, int64_t stride, int64_t T, int 
   double* part = (double*)ws;
   unsigned* ticket = (unsigned*)(part + kMaxExperts / kJoinExperts);
   float* sums = (float*)(ticket + 4);
-  const size_t lds = sizeof(int) * (size_t)(E + 1 + kPartWaves * E);
+  size_t lds = sizeof(int) * (size_t)(E + 1 + kPartWaves * E);
+  if (lds < sizeof(double) * kPartWaves * 4) lds = sizeof(double) * kPartWaves * 4;
   const auto go = [&](auto zero, auto v, auto nj, auto g) {
     typedef decltype(zero) TT;
     hipLaunchKernelGGL((balance_part_k<TT, decltype(v)::value, decltype(nj)::value, decltype(g)::value>), dim3(blocks),
-                       dim3(kPartThreads), lds, st, (const TT*)x, stride, T, E, idx, k, valid, kind, rows, sums, ticket);
+                       dim3(kPartThreads), lds, st, (const TT*)x, stride, T, E, idx, k, valid, kind, rows, sums, ticket, counts);
   };
   if (is_bf16) with_plan<8>(r, [&](auto v, auto nj, auto g) { go(bf16(), v, nj, g); });
   else with_plan<4>(r, [&](auto v, auto nj, auto g) { go(0.f, v, nj, g); });
   HETU_LAUNCH_CHECK();
-  hipLaunchKernelGGL(balance_join_k, dim3((E + kJoinExperts - 1) / kJoinExperts), dim3(kJoinThreads), 0, st, sums,
+  if (blocks > 1)
+    hipLaunchKernelGGL(balance_join_k, dim3((E + kJoinExperts - 1) / kJoinExperts), dim3(kJoinThreads), 0, st, sums,
                      blocks, E, counts, weight, loss, part, ticket);
   HETU_LAUNCH_CHECK();
   return 0;
@@ -466,6 +505,8 @@ HETU_API int hetu_moe_balance_bwd(const void* x, int64_t stride, int64_t T, int 
   const RowPlan r = plan_rows(E, stride, x, dx, is_bf16 ? 8 : 4);
   const int64_t groups = kBlThreads / r.G * (r.NJ * r.V <= 8 ? 2 : 1);
   const int64_t want = (T + groups - 1) / groups;
+  // 8 blocks a CU loop over the rows, for each block reads the weights: 262144 x 256 bf16 57 us, with
+  // 8192 blocks 75, with one for each of its rows 122
   const dim3 grid((unsigned)(want < 2048 ? want : 2048));
   const auto go = [&](auto zero, auto v, auto nj, auto g) {
     typedef decltype(zero) TT;

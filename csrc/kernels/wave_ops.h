@@ -54,6 +54,24 @@ __device__ __forceinline__ float group_sum(float v, int G) {
   }));
 }
 
+// sum over the lanes of a wave with the same place in their group of G
+template <int G>
+__device__ __forceinline__ float place_sum(float v) {
+#pragma clang fp contract(off)
+  const auto add = [](unsigned a, unsigned b) {
+#pragma clang fp contract(off)
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  };
+  unsigned b = __float_as_uint(v);
+  if constexpr (G < 2) b = lane_join<1>(b, add);
+  if constexpr (G < 4) b = lane_join<2>(b, add);
+  if constexpr (G < 16) b = add(b, dpp<0x128>(b));       // row_ror:8
+  if constexpr (G < 8) b = add(b, dpp<0x124>(b));        // row_ror:4
+  if constexpr (G < 32) b = lane_join<16>(b, add);
+  if constexpr (G < 64) b = lane_join<32>(b, add);
+  return __uint_as_float(b);
+}
+
 // sum over the lanes with the same place in their quad (16 of a wave), of a 64-bit number or double
 template <typename T>
 __device__ __forceinline__ T quad_place_sum(T v) {

@@ -7,9 +7,11 @@ import math
 import torch
 from .. import native_array as _NA
 
-from . import fn, native, stream_ptr, is_bf16, check, check_device, supported_float, record_native, P, I64, I32
+from . import fn, native, stream_ptr, is_bf16, check, check_device, ptr, supported_float, record_native, P, I64, I32
 
 MAX_TOP = 64
+_FWD = [P, I64, P, I64, I32, I32, I64, P, P, I32, P]
+_BWD = [P, I64, P, I64, I32, I32, I64, P, P, P, P, I32, P]
 
 
 class TokenLogProb(object):
@@ -17,10 +19,16 @@ class TokenLogProb(object):
     ``top_logp`` [..., top], all columns of ``out`` (fp32 [..., 2 + top]); ``top_ids`` [..., top]
     (int64); ``stats`` [..., 2], each row's maximum and base-2 log of its sum, for the backward
     pass.  The fp32 parts are views of one buffer [..., 4 + top]."""
-    __slots__ = ('buffer', 'top_ids')
+    __slots__ = ('buffer', 'ids')
 
-    def __init__(self, buffer, top_ids):
-        self.buffer, self.top_ids = buffer, top_ids
+    def __init__(self, buffer, ids):
+        self.buffer, self.ids = buffer, ids
+
+    @property
+    def top_ids(self):
+        if self.ids is None:           # no alternatives
+            return self.buffer.new_empty(self.buffer.shape[:-1] + (0,), dtype=torch.int64)
+        return self.ids
 
     @property
     def top(self):
@@ -55,16 +63,18 @@ def _operands(name, logits, ids, top):
         raise ValueError('%s: a row has 1 to 2^31 - 65 logits, got %d' % (name, V))
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError('%s: top is 0 to min(%d, %d), got %d' % (name, MAX_TOP, V, top))
-    lead = tuple(logits.shape[:-1])
-    R = math.prod(lead)
+    two = logits.dim() == 2
+    lead = (logits.shape[0],) if two else tuple(logits.shape[:-1])
+    R = lead[0] if two else math.prod(lead)
     if ids.numel() != R or ids.is_floating_point() and ids.dtype not in (torch.float32, torch.float64):
         raise ValueError('%s: one token id a row: %d rows, ids %s %s' % (name, R, tuple(ids.shape), ids.dtype))
     if ids.device != logits.device:
         raise ValueError('%s: logits on %s, ids on %s' % (name, logits.device, ids.device))
-    x = logits.reshape(R, V) if logits.dim() != 2 else logits
-    if V > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < 0:
+    x = logits if two else logits.reshape(R, V)
+    if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    ids = ids.reshape(R)
+    if ids.dim() != 1:
+        ids = ids.reshape(R)
     if ids.dtype != torch.int64:
         ids = ids.long()
     return x, ids.contiguous(), lead, R, V
@@ -84,14 +94,14 @@ def token_logprob(logits, ids, top=0, ignored_index=-1):
     A NaN or +inf makes its row NaN."""
     x, ids, lead, R, V = _operands('token_logprob', logits, ids, top)
     r = TokenLogProb(_NA.empty(lead + (4 + top,), dtype=torch.float32, device=x.device),
-                     _NA.empty(lead + (top,), dtype=torch.int64, device=x.device))
+                     _NA.empty(lead + (top,), dtype=torch.int64, device=x.device) if top else None)
     if R == 0:
         return r
     if native(x):
         check_device(x, 'token_logprob')
-        f = fn('hetu_token_logprob', [P, I64, P, I64, I32, I32, I64, P, P, I32, P])
-        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, ignored_index, r.buffer.data_ptr(),
-                r.top_ids.data_ptr(), is_bf16(x), stream_ptr()), 'token_logprob')
+        f = fn('hetu_token_logprob', _FWD)
+        check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, ignored_index, r.buffer.data_ptr(), ptr(r.ids),
+                is_bf16(x), stream_ptr()), 'token_logprob')
         record_native('token_logprob')
         return r
     xf = x.float()
@@ -135,10 +145,9 @@ def token_logprob_backward(logits, ids, fwd, grad, ignored_index=-1):
         return dx
     if native(x):
         check_device(x, 'token_logprob_backward')
-        f = fn('hetu_token_logprob_bwd', [P, I64, P, I64, I32, I32, I64, P, P, P, P, I32, P])
+        f = fn('hetu_token_logprob_bwd', _BWD)
         check(f(x.data_ptr(), _stride(x), ids.data_ptr(), R, V, top, ignored_index, fwd.buffer.data_ptr(),
-                fwd.top_ids.data_ptr(), grad.data_ptr(), dx.data_ptr(), is_bf16(x), stream_ptr()),
-              'token_logprob_bwd')
+                ptr(fwd.ids), grad.data_ptr(), dx.data_ptr(), is_bf16(x), stream_ptr()), 'token_logprob_bwd')
         record_native('token_logprob_bwd')
         return dx
     g, o = grad.reshape(R, 2 + top), fwd.out.reshape(R, 2 + top)

@@ -109,6 +109,8 @@ def aux_terms(counts, psum, T):
 
 # ---- balance loss with counts (moe_balance.hip) --------------------------------------------------
 MAX_EXPERTS = 1024
+_BALANCE_FWD = [P, I64, I64, I32, P, I32, P, I32, P, P, I32, P]
+_BALANCE_BWD = [P, I64, I64, I32, P, P, P, I32, P, I32, P]
 _VALID_KINDS = {torch.bool: 0, torch.uint8: 0, torch.int8: 0, torch.float32: 1, torch.bfloat16: 2, torch.int64: 3,
                 torch.int32: 4}
 
@@ -147,13 +149,14 @@ def _balance_operands(name, logits, valid):
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError('%s: 1 to %d experts, got %d' % (name, MAX_EXPERTS, E))
     x = logits
-    if E > 1 and x.stride(1) != 1 or T > 1 and x.stride(0) < 0:
+    if E > 1 and x.stride(1) != 1:
         x = _dc(x)
     if valid is not None:
         if valid.numel() != T or valid.dtype not in _VALID_KINDS or valid.device != x.device:
             raise ValueError('%s: valid has to hold one value a token (%d) on %s, got %s %s on %s'
                              % (name, T, x.device, valid.dtype, tuple(valid.shape), valid.device))
-        valid = _dc(valid).reshape(T)
+        if not valid.is_contiguous():
+            valid = _dc(valid)
     return x, valid, T, E
 
 
@@ -170,7 +173,9 @@ def balance_loss(logits, indices, num_experts, valid=None):
     if indices.dim() < 1 or indices.shape[0] != T or T and indices.numel() % T or indices.device != x.device:
         raise ValueError('balance_loss: indices have to be [%d, k] on %s, got %s on %s'
                          % (T, x.device, tuple(indices.shape), indices.device))
-    idx = indices.reshape(T, -1) if indices.numel() else indices.reshape(T, 0)
+    idx = indices
+    if idx.dim() != 2:
+        idx = idx.reshape(T, -1) if idx.numel() else idx.reshape(T, 0)
     k = idx.shape[1]
     if T and k < 1:
         raise ValueError('balance_loss: at least one choice a token')
@@ -181,14 +186,14 @@ def balance_loss(logits, indices, num_experts, valid=None):
         idx = _dc(idx)
         r = BalanceLoss(_NA.empty((E + E // 2 + 1,), dtype=torch.int64, device=x.device), E)
         ws = _NA.empty((_balance_ws(T, E),), dtype=torch.int32, device=x.device)
-        f = fn('hetu_moe_balance_fwd', [P, I64, I64, I32, P, I32, P, I32, P, P, I32, P])
+        f = fn('hetu_moe_balance_fwd', _BALANCE_FWD)
         check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, idx.data_ptr(), max(k, 1), ptr_or_none(valid),
                 _VALID_KINDS[valid.dtype] if valid is not None else 0, r.buffer.data_ptr(), ws.data_ptr(), is_bf16(x),
                 stream_ptr()), 'moe_balance')
         record_native('moe_balance')
         return r
     r = BalanceLoss(torch.zeros(E + E // 2 + 1, dtype=torch.int64, device=x.device), E)
-    on = torch.ones(T, dtype=torch.bool, device=x.device) if valid is None else valid != 0
+    on = torch.ones(T, dtype=torch.bool, device=x.device) if valid is None else valid.reshape(T) != 0
     chosen = idx[on].reshape(-1)
     chosen = chosen[(chosen >= 0) & (chosen < E)]
     r.counts.copy_(torch.bincount(chosen, minlength=E))
@@ -212,7 +217,7 @@ def balance_loss_backward(logits, fwd, grad, valid=None):
         check_device(x, 'balance_loss_backward')
         grad = _dc(grad, torch.float32)
         dx = _NA.empty((T, E), dtype=x.dtype, device=x.device)
-        f = fn('hetu_moe_balance_bwd', [P, I64, I64, I32, P, P, P, I32, P, I32, P])
+        f = fn('hetu_moe_balance_bwd', _BALANCE_BWD)
         check(f(x.data_ptr(), x.stride(0) if T > 1 else E, T, E, fwd.buffer.data_ptr() + 8 * E,
                 grad.data_ptr(), ptr_or_none(valid), _VALID_KINDS[valid.dtype] if valid is not None else 0, dx.data_ptr(), is_bf16(x),
                 stream_ptr()), 'moe_balance_bwd')
@@ -221,7 +226,7 @@ def balance_loss_backward(logits, fwd, grad, valid=None):
     p = torch.softmax(x.float(), 1)
     d = grad.float().reshape(1, 1) * p * (fwd.weight - (p * fwd.weight).sum(1, keepdim=True))
     if valid is not None:
-        d = torch.where((valid != 0)[:, None], d, torch.zeros_like(d))
+        d = torch.where((valid.reshape(T) != 0)[:, None], d, torch.zeros_like(d))
     return d.to(x.dtype)
 
 

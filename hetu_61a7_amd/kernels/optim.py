@@ -74,6 +74,7 @@ def optimizer_flat(mode, p, g, s1=None, s2=None, shadow=None, lr=0.01, l2=0.0, m
 
 
 # ---- AdamW with both moments in 8 bits (adamw8.hip) ---------------------------------------------
+_ADAMW8 = [P, P, P, P, P, P, P, I64] + [F32] * 10 + [P, I64, P]
 STATE8_BLOCK = 256      # consecutive elements that share the moments' scales
 
 
@@ -171,7 +172,7 @@ def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.
         return
     if native(p):
         check_device(p, 'adamw8')
-        f = fn('hetu_adamw8', [P, P, P, P, P, P, P, I64] + [F32] * 10 + [P, I64, P])
+        f = fn('hetu_adamw8', _ADAMW8)
         check(f(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale.data_ptr(), v_scale.data_ptr(),
                 ptr(shadow), n, lr, beta1, beta2, 1.0 - beta1, 1.0 - beta2, 1.0 - beta1t, 1.0 - beta2t, eps,
                 wd, gscale, ptr(dyn), _i64(seed), stream_ptr()), 'adamw8')
