@@ -208,7 +208,7 @@ HETU_API int hetu_adamw8(float* p, const float* g, void* m, void* v, float* ms, 
   // a block of 8 half waves for each 8 blocks of elements: 109 M weights take 345 us, with 2048 that
   // loop over them 389 (they load and store in step), with non-temporal accesses 395 to 405
   const int64_t want = (nb + 7) / 8;
-  const dim3 grid((unsigned)(want < 0x7fffffff ? want : 0x7fffffff));
+  const dim3 grid((unsigned)(want < 1 << 22 ? want : 1 << 22));     // 8.6e9 elements; more: a loop
   const bool vec = (((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)m | (uintptr_t)v) & 7) == 0 &&
                    ((uintptr_t)shadow & 15) == 0;
 #define GO(S, V) hipLaunchKernelGGL((adamw8_k<S, V>), grid, dim3(256), 0, st, p, g, (unsigned char*)m, (unsigned char*)v, \

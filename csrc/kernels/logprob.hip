@@ -25,6 +25,14 @@ namespace hetu {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMaxTop = 64;
 
+// A launch holds fewer than 2^32 threads along x: more blocks than kRowOfBlocks go along y too.
+constexpr int64_t kRowOfBlocks = 1 << 20;
+constexpr int64_t kMaxBlocks = kRowOfBlocks * 65535;
+static dim3 many_blocks(int64_t n) {
+  return n <= kRowOfBlocks ? dim3((unsigned)n) : dim3((unsigned)kRowOfBlocks, (unsigned)((n + kRowOfBlocks - 1) / kRowOfBlocks));
+}
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * kRowOfBlocks + blockIdx.x; }
+
 struct Lse { float m, s, u; };       // running maximum, sum, base-2 weighted sum
 
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f : m; }
@@ -138,8 +146,9 @@ __device__ __forceinline__ void lse_take(Lse& a, int& best, const float (&v)[U][
 // them under way at once; thread 0 the head and the last thread the tail that are not whole.
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
-                                                      const int64_t* __restrict__ ids, int V, int n, int64_t ignored,
-                                                      float* __restrict__ out, int64_t* __restrict__ top) {
+                                                      const int64_t* __restrict__ ids, int64_t R, int V, int n,
+                                                      int64_t ignored, float* __restrict__ out,
+                                                      int64_t* __restrict__ top) {
   constexpr int VE = Vec<T>::N, U = 4, NW = NT / 64;
   constexpr int NG = TOP ? (NT < 256 ? NT : 256) : 1, PER = TOP ? NT / NG : 1;   // groups of threads that give a sample
   constexpr int CAND = NT < 256 ? 512 : 1024;       // candidates kept in LDS; more take the slow way
@@ -147,7 +156,8 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
   __shared__ uint64_t keys[NG], cand[TOP ? CAND : 1], bound;
   __shared__ int flagged[NG], n_flagged, n_cand;
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_number();
+  if (row >= R) return;
   float* o = out + row * (4 + n);
   const Row<T> r(logits + row * stride, V);
   int j = r.f0 + tid;
@@ -338,16 +348,17 @@ constexpr int kBwdThreads = 256, kBwdU = 4, kBwdGranules = kBwdThreads * kBwdU *
 
 template <typename T>
 __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __restrict__ logits, int64_t stride,
-                                                                   const int64_t* __restrict__ ids, int V, int n,
-                                                                   int64_t ignored, int chunks,
+                                                                   const int64_t* __restrict__ ids, int64_t R, int V,
+                                                                   int n, int64_t ignored, int chunks,
                                                                    const float* __restrict__ out,
                                                                    const int64_t* __restrict__ top,
                                                                    const float* __restrict__ grad, T* __restrict__ dx) {
   constexpr int NT = kBwdThreads, VE = Vec<T>::N, U = kBwdU;
   const int tid = threadIdx.x;
-  const unsigned at = gridDim.x - 1 - blockIdx.x;
+  const int64_t at = R * chunks - 1 - block_number();
+  if (at < 0) return;
   const int64_t row = at / chunks;
-  const int chunk = at % chunks;
+  const int chunk = (int)(at - row * chunks);
   const int64_t t = ids[row];
   T* d = dx + row * (int64_t)V;
   const float* o = out + row * (4 + n);
@@ -436,8 +447,8 @@ using namespace hetu;
 template <typename T>
 static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, int64_t R, int V, int n, int64_t ignored,
                        float* out, int64_t* top, hipStream_t st) {
-#define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), dim3((unsigned)R), dim3(NT), 0, st, \
-                                       (const T*)logits, stride, ids, V, n, ignored, out, top)
+#define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), many_blocks(R), dim3(NT), 0, st, \
+                                       (const T*)logits, stride, ids, R, V, n, ignored, out, top)
   const int64_t bytes = (int64_t)V * sizeof(T);
   // a wave a row up to 4 KB; 1024 threads for long rows that are few, or that have alternatives to
   // find (a thread's elements are read again: 1000 x 131072 top 20 63 us, with 256 threads 71); 256
@@ -454,7 +465,7 @@ HETU_API int hetu_token_logprob(const void* logits, int64_t stride, const int64_
                                 int64_t ignored, float* out, int64_t* top, int is_bf16,
                                 hipStream_t st) {
   if (R <= 0) return 0;
-  if (V < 1 || n < 0 || n > kMaxTop || n > V || R > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (V < 1 || n < 0 || n > kMaxTop || n > V || R > kMaxBlocks) return (int)hipErrorInvalidValue;
   if (is_bf16) launch_fwd<bf16>(logits, stride, ids, R, V, n, ignored, out, top, st);
   else launch_fwd<float>(logits, stride, ids, R, V, n, ignored, out, top, st);
   HETU_LAUNCH_CHECK();
@@ -467,12 +478,12 @@ HETU_API int hetu_token_logprob_bwd(const void* logits, int64_t stride, const in
   if (R <= 0) return 0;
   const int VE = is_bf16 ? 8 : 4;
   const int64_t chunks = ((int64_t)V + 2 * VE - 2 + (int64_t)VE * kBwdGranules - 1) / ((int64_t)VE * kBwdGranules);
-  if (V < 1 || n < 0 || n > kMaxTop || n > V || R * chunks > 0x7fffffff) return (int)hipErrorInvalidValue;
-  const dim3 grid((unsigned)(R * chunks)), block(kBwdThreads);
+  if (V < 1 || n < 0 || n > kMaxTop || n > V || R > kMaxBlocks / chunks) return (int)hipErrorInvalidValue;
+  const dim3 grid = many_blocks(R * chunks), block(kBwdThreads);
   if (is_bf16)
-    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, V, n, ignored, (int)chunks, out, top, grad, (bf16*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, R, V, n, ignored, (int)chunks, out, top, grad, (bf16*)dx);
   else
-    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, V, n, ignored, (int)chunks, out, top, grad, (float*)dx);
+    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, R, V, n, ignored, (int)chunks, out, top, grad, (float*)dx);
   HETU_LAUNCH_CHECK();
   return 0;
 }

@@ -89,7 +89,7 @@ def check(ret, name=''):
 
 def check_device(t, name=''):
     """a launch goes to the current device: tensors of another one are refused, not read from it"""
-    if t.device.index != torch.cuda.current_device():
+    if t.device.index != torch._C._cuda_getDevice():
         raise ValueError('%s: tensors on %s, but the current device is cuda:%d'
                          % (name, t.device, torch.cuda.current_device()))
 

@@ -130,11 +130,11 @@ class BalanceLoss(object):
 
     @property
     def weight(self):
-        return self.buffer[self.experts:].view(torch.float32)[:self.experts]
+        return self.buffer.view(torch.float32)[2 * self.experts:3 * self.experts]
 
     @property
     def loss(self):
-        return self.buffer[self.experts:].view(torch.float32)[self.experts:self.experts + 1]
+        return self.buffer.view(torch.float32)[3 * self.experts:3 * self.experts + 1]
 
 
 @functools.lru_cache(maxsize=4096)

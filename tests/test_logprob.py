@@ -256,6 +256,22 @@ def test_same_call_gives_the_same_bits_and_another_stream():
     assert torch.equal(r.out, r2.out) and torch.equal(r.top_ids, r2.top_ids) and torch.equal(d, d2)
 
 
+@pytest.mark.gpu
+def test_more_rows_than_one_dimension_of_a_launch_holds():
+    """2^24 + 5 rows of 3 logits: 2^32 threads in the backward pass"""
+    R = (1 << 24) + 5
+    x = torch.randn(R, 3, device='cuda').to(torch.bfloat16)
+    ids = torch.arange(R, device='cuda') % 3
+    grad = torch.ones(R, 2, device='cuda')
+    grad[:, 1] = 0
+    r = K.token_logprob(x, ids)
+    d = K.token_logprob_backward(x, ids, r, grad)
+    for a, b in ((0, 1000), ((1 << 20) - 500, (1 << 20) + 500), ((1 << 24) - 500, R)):
+        s = slice(a, b)
+        part = K.TokenLogProb(r.buffer[s], None)
+        _check(x[s], ids[s], 0, torch.bfloat16, part, d[s], grad[s])
+
+
 # ---- as graph operators ------------------------------------------------------------------------
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('graph', [False, True])
