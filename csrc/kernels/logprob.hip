@@ -144,16 +144,19 @@ __device__ __forceinline__ void lse_take(Lse& a, int& best, const float (&v)[U][
 
 // One block of NT threads a row: thread i takes the whole granules f0 + i, f0 + i + NT, .., U of
 // them under way at once; thread 0 the head and the last thread the tail that are not whole.
+// (More than 80 scalar registers leave a SIMD 7 waves, and a CU one block of 1024 threads instead of
+// two: 1000 x 131072 top 20 took 80 us instead of 62.)
 template <typename T, int NT, bool TOP>
-__global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
+__attribute__((amdgpu_num_sgpr(80))) __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logits, int64_t stride,
                                                       const int64_t* __restrict__ ids, int64_t R, int V, int n,
                                                       int64_t ignored, float* __restrict__ out,
                                                       int64_t* __restrict__ top) {
   constexpr int VE = Vec<T>::N, U = 4, NW = NT / 64;
-  constexpr int NG = TOP ? (NT < 256 ? NT : 256) : 1, PER = TOP ? NT / NG : 1;   // groups of threads that give a sample
-  constexpr int CAND = NT < 256 ? 512 : 1024;       // candidates kept in LDS; more take the slow way
+  constexpr int NG = TOP ? 256 : 1, PER = TOP ? NT / NG : 1;   // groups of threads that give a sample
+  constexpr int CAND = 1024;                        // candidates kept in LDS; more take the slow way
   __shared__ Lse part[NW];
-  __shared__ uint64_t keys[NG], cand[TOP ? CAND : 1], bound;
+  __shared__ __align__(16) uint64_t cand[TOP ? CAND + 1 : 1];
+  __shared__ uint64_t keys[NG], bound;
   __shared__ int flagged[NG], n_flagged, n_cand;
   const int tid = threadIdx.x;
   const int64_t row = block_number();
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
   uint64_t mine = 0;                  // this thread's sample; 0: it has no element
   if (TOP && best >= 0) mine = key_of(a.m, best);
   a = lse_join(a, 64);
-  if (NW > 1 && (tid & 63) == 0) part[tid >> 6] = a;
+  if ((tid & 63) == 0) part[tid >> 6] = a;
   if (TOP) {
 #pragma unroll
     for (int s = 1; s < PER; s <<= 1) {
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     if (tid == 0) { n_flagged = 0; n_cand = 0; }
   }
   __syncthreads();
-  if (NW > 1) a = lse_join(part[tid & (NW - 1)], NW);
+  a = lse_join(part[tid & (NW - 1)], NW);
   const bool empty = a.m == -INFINITY && a.s == 0.f;
   const float log2s = log2f(a.s), logs = log2s * kLn2;
   if (tid == NT - 1) {
@@ -299,10 +302,18 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
     __syncthreads();
     const int C = n_cand;
     if (C <= CAND) {
+      if (C & 1) {                 // read in pairs
+        if (tid == 0) cand[C] = 0;
+        __syncthreads();
+      }
       for (int c = tid; c < C; c += NT) {
         const uint64_t key = cand[c];
         int at = 0;
-        for (int i = 0; i < C; ++i) at += cand[i] > key;
+#pragma unroll 4
+        for (int i = 0; i < C; i += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&cand[i]);
+          at += (two.x > key) + (two.y > key);
+        }
         if (at < n) {
           o[2 + at] = empty ? -INFINITY : (key_value(key) - a.m) - logs;
           top[row * n + at] = key_index(key);
@@ -338,6 +349,141 @@ __global__ void __launch_bounds__(NT) token_logprob_k(const T* __restrict__ logi
         o[2 + i] = empty ? -INFINITY : (key_value(most) - a.m) - logs;
         top[row * n + i] = key_index(most);
       }
+    }
+  }
+}
+
+// ---- rows of at most kShortBytes: a wave a row, held in registers ----------------------------
+constexpr int kShortBytes = 4080, kShortGranules = 4;      // at most 256 granules with the head's: 4 a lane
+constexpr int kShortWaves = 4;
+
+// sorts one key a lane, the largest first
+__device__ __forceinline__ uint64_t wave_sort(uint64_t key, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)key, d, 64);
+      const bool larger = ((lane & d) == 0) == ((lane & size) == 0);      // this lane keeps the larger one
+      key = (key > other) == larger ? key : other;
+    }
+  return key;
+}
+
+// the largest number that n of the wave's keys k reach, or one between the n-th and the next; 0 where
+// they are fewer
+template <int Q>
+__device__ __forceinline__ uint64_t nth_bound(const uint64_t (&k)[Q], int n) {
+  uint64_t b = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t c = b | (1ull << bit);
+    int reach = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(k[q] >= c));
+    if (reach >= n) b = c;
+    if (reach == n) break;
+  }
+  return b;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const T* __restrict__ logits, int64_t stride,
+                                                                          const int64_t* __restrict__ ids, int64_t R,
+                                                                          int V, int n, int64_t ignored,
+                                                                          float* __restrict__ out,
+                                                                          int64_t* __restrict__ top) {
+  constexpr int VE = Vec<T>::N, Q = kShortGranules, CAND = kMaxTop * VE, K = CAND / 64;
+  __shared__ uint64_t found[kShortWaves][TOP ? CAND : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = block_number() * kShortWaves + wave;
+  if (row >= R) return;
+  float* o = out + row * (4 + n);
+  const int64_t t = ids[row];
+  if (t < 0 || t >= V || t == ignored) {
+    for (int i = lane; i < 4 + n; i += 64) o[i] = 0.f;
+    for (int i = lane; i < n; i += 64) top[row * n + i] = -1;
+    return;
+  }
+  const Row<T> r(logits + row * stride, V);
+  const float xt = to_f(r.x[t]);
+  float v[Q][VE];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) r.load(lane + 64 * q, v[q]);        // -inf beyond the row
+  uint64_t k[Q];
+  float m = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    float vm = v[q][0];
+#pragma unroll
+    for (int e = 1; e < VE; ++e) vm = fmaxf(vm, v[q][e]);
+    if (TOP) k[q] = lane + 64 * q < r.ng ? key_of(vm, lane + 64 * q) : 0;
+    m = fmaxf(m, vm);
+  }
+  Lse a = {group_max(m, 64), 0.f, 0.f};
+  const float sh = shift_of(a.m);
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float d = (v[q][e] - sh) * kLog2e, x = exp2_(d);
+      a.s += x;
+      a.u += x * fmaxf(d, kFloor2);
+    }
+  a.s = group_sum(a.s, 64);
+  a.u = group_sum(a.u, 64);
+  const bool empty = a.m == -INFINITY && a.s == 0.f;
+  const float log2s = log2f(a.s), logs = log2s * kLn2;
+  if (lane == 0) {
+    o[0] = empty ? -INFINITY : (xt - a.m) - logs;
+    o[1] = empty ? 0.f : (log2s - a.u / a.s) * kLn2;
+    o[2 + n] = a.m;
+    o[3 + n] = log2s;
+  }
+  if constexpr (TOP) {
+    // the granules of the n largest samples, or all where they are fewer: at most 64 VE elements
+    const uint64_t least = nth_bound<Q>(k, n), below = (1ull << lane) - 1;
+    uint64_t* cand = found[wave];
+    int C = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int j = lane + 64 * q, e0 = j * VE - r.off;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const bool in = k[q] != 0 && k[q] >= least && e0 + e >= 0 && e0 + e < V && key_of(v[q][e], j) >= least;
+        const uint64_t mask = __ballot(in);
+        if (in) cand[C + __popcll(mask & below)] = key_of(v[q][e], e0 + e);
+        C += __popcll(mask);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    uint64_t key = 0;
+    if (C <= 64) {
+      if (lane < C) key = cand[lane];
+    } else {                       // more than a wave sorts: the n largest of them
+      uint64_t c[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) c[i] = lane + 64 * i < C ? cand[lane + 64 * i] : 0;
+      const uint64_t bound = nth_bound<K>(c, n);
+      __builtin_amdgcn_wave_barrier();
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const bool in = c[i] >= bound;
+        const uint64_t mask = __ballot(in);
+        if (in) cand[at + __popcll(mask & below)] = c[i];
+        at += __popcll(mask);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if (lane < n) key = cand[lane];
+    }
+    key = wave_sort(key, lane);
+    if (lane < n) {
+      o[2 + lane] = empty ? -INFINITY : (key_value(key) - a.m) - logs;
+      top[row * n + lane] = key_index(key);
     }
   }
 }
@@ -450,12 +596,18 @@ static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, i
 #define GO(NT, TOP) hipLaunchKernelGGL((token_logprob_k<T, NT, TOP>), many_blocks(R), dim3(NT), 0, st, \
                                        (const T*)logits, stride, ids, R, V, n, ignored, out, top)
   const int64_t bytes = (int64_t)V * sizeof(T);
-  // a wave a row up to 4 KB; 1024 threads for long rows that are few, or that have alternatives to
-  // find (a thread's elements are read again: 1000 x 131072 top 20 63 us, with 256 threads 71); 256
-  // threads else (8192 x 30522 117 us, with 128 130, with 512 124)
-  if (bytes <= 4096) { if (n) GO(64, true); else GO(64, false); }
-  else if (bytes >= 32768 && (R <= 512 || n)) { if (n) GO(1024, true); else GO(1024, false); }
-  else { if (n) GO(256, true); else GO(256, false); }
+  // 1024 threads for long rows that are few, or that have alternatives to find (a thread's elements are
+  // read again: 1000 x 131072 top 20 63 us, with 256 threads 71); 256 threads else (8192 x 30522 117
+  // us, with 128 130, with 512 124); a wave for rows that it holds in registers
+  if (bytes <= kShortBytes) {
+    const dim3 grid = many_blocks((R + kShortWaves - 1) / kShortWaves), block(64 * kShortWaves);
+    if (n) hipLaunchKernelGGL((token_logprob_short_k<T, true>), grid, block, 0, st, (const T*)logits, stride, ids, R, V, n, ignored, out, top);
+    else hipLaunchKernelGGL((token_logprob_short_k<T, false>), grid, block, 0, st, (const T*)logits, stride, ids, R, V, n, ignored, out, top);
+  } else if (bytes >= 32768 && (R <= 512 || n)) {
+    if (n) GO(1024, true); else GO(1024, false);
+  } else {
+    if (n) GO(256, true); else GO(256, false);
+  }
 #undef GO
 }
 
