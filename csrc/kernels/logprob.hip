@@ -113,6 +113,58 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)~(unsigned)key; }
 
+// A bound that n of the wave's keys k reach and, but for fewer keys than n (then 0), no more: found
+// two bits at a time from the highest that differs, first by the values (of which LOW bits are the
+// same in a sign: bf16), then where they tie by the low words, ~0 .. ~(limit - 1).
+template <int Q, int LOW>
+__device__ __forceinline__ uint64_t nth_bound(const uint64_t (&k)[Q], int n, unsigned limit) {
+  unsigned hi[Q], most = 0, least = ~0u;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    hi[q] = (unsigned)(k[q] >> 32);
+    most = most > hi[q] ? most : hi[q];
+    least = least < hi[q] ? least : hi[q];
+  }
+  most = group_join(most, 64, [](unsigned a, unsigned b) { return a > b ? a : b; });
+  least = group_join(least, 64, [](unsigned a, unsigned b) { return a < b ? a : b; });
+  most = (unsigned)__builtin_amdgcn_readfirstlane((int)most);       // (uniform: in scalar registers)
+  least = (unsigned)__builtin_amdgcn_readfirstlane((int)least);
+  const unsigned differ = most ^ least;
+  int at = differ ? (31 - __builtin_clz(differ)) & ~1 : -2, reach = -1;
+  unsigned b = differ ? (most >> at >> 2) << at << 2 | ((most & least) & (2u << at)) : most;
+  for (; at >= LOW && reach != n; at -= 2) {
+    const unsigned c1 = b | 1u << at, c2 = b | 2u << at, c3 = b | 3u << at;
+    int r1 = 0, r2 = 0, r3 = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      r1 += __popcll(__ballot(hi[q] >= c1));
+      r2 += __popcll(__ballot(hi[q] >= c2));
+      r3 += __popcll(__ballot(hi[q] >= c3));
+    }
+    if (r3 >= n) b = c3, reach = r3;
+    else if (r2 >= n) b = c2, reach = r2;
+    else if (r1 >= n) b = c1, reach = r1;
+  }
+  if (reach == n) return (uint64_t)b << 32;
+  if (LOW && !(b >> 31)) b |= (1u << LOW) - 1;       // below 0 the same bits are ones
+  at = (31 - __builtin_clz(limit | 1)) & ~1;
+  uint64_t w = (uint64_t)b << 32 | (at >= 30 ? 0u : ~0u << at << 2);
+  for (; at >= 0 && reach != n; at -= 2) {
+    const uint64_t c1 = w | 1u << at, c2 = w | 2u << at, c3 = w | 3u << at;
+    int r1 = 0, r2 = 0, r3 = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      r1 += __popcll(__ballot(k[q] >= c1));
+      r2 += __popcll(__ballot(k[q] >= c2));
+      r3 += __popcll(__ballot(k[q] >= c3));
+    }
+    if (r3 >= n) w = c3, reach = r3;
+    else if (r2 >= n) w = c2, reach = r2;
+    else if (r1 >= n) w = c1, reach = r1;
+  }
+  return w;
+}
+
 // takes U granules v (numbers j, j + step, ..) into the running sums; `best`: the granule with the
 // first of the largest values so far
 template <int U, int VE, bool TOP>
@@ -241,34 +293,12 @@ __attribute__((amdgpu_num_sgpr(80))) __global__ void __launch_bounds__(NT) token
     o[3 + n] = log2s;
   }
   if constexpr (TOP) {
-    // the n-th largest sample, bit by bit from the highest: the largest key that n samples reach (0
-    // where fewer than n threads have an element: then all are candidates)
+    // the n-th largest sample (0 where fewer than n threads have an element: all are candidates)
     if (tid < 64) {
-      constexpr int Q = NG / 64;
-      unsigned hi[Q];
-      uint64_t k[Q], b = 0;
-      unsigned bh = 0;
-      int reach = 0;
+      uint64_t k[NG / 64];
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        k[q] = keys[tid + q * 64];
-        hi[q] = (unsigned)(k[q] >> 32);
-      }
-      for (int bit = 31; bit >= 0 && reach != n; --bit) {          // by the values,
-        const unsigned c = bh | (1u << bit);
-        reach = 0;
-#pragma unroll
-        for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(hi[q] >= c));
-        if (reach >= n) bh = c;
-      }
-      b = (uint64_t)bh << 32;
-      for (int bit = 31; bit >= 0 && reach != n; --bit) {          // and where they tie by the granules
-        const uint64_t c = b | (1u << bit);
-        reach = 0;
-#pragma unroll
-        for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(k[q] >= c));
-        if (reach >= n) b = c;
-      }
+      for (int q = 0; q < NG / 64; ++q) k[q] = keys[tid + q * 64];
+      const uint64_t b = nth_bound<NG / 64, sizeof(T) == 2 ? 16 : 0>(k, n, r.ng);
       if (tid == 0) bound = b;
     }
     __syncthreads();
@@ -370,22 +400,6 @@ __device__ __forceinline__ uint64_t wave_sort(uint64_t key, int lane) {
   return key;
 }
 
-// the largest number that n of the wave's keys k reach, or one between the n-th and the next; 0 where
-// they are fewer
-template <int Q>
-__device__ __forceinline__ uint64_t nth_bound(const uint64_t (&k)[Q], int n) {
-  uint64_t b = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t c = b | (1ull << bit);
-    int reach = 0;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) reach += __popcll(__ballot(k[q] >= c));
-    if (reach >= n) b = c;
-    if (reach == n) break;
-  }
-  return b;
-}
-
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const T* __restrict__ logits, int64_t stride,
                                                                           const int64_t* __restrict__ ids, int64_t R,
@@ -441,7 +455,7 @@ __global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const 
   }
   if constexpr (TOP) {
     // the granules of the n largest samples, or all where they are fewer: at most 64 VE elements
-    const uint64_t least = nth_bound<Q>(k, n), below = (1ull << lane) - 1;
+    const uint64_t least = nth_bound<Q, sizeof(T) == 2 ? 16 : 0>(k, n, r.ng), below = (1ull << lane) - 1;
     uint64_t* cand = found[wave];
     int C = 0;
 #pragma unroll
@@ -465,12 +479,12 @@ __global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const 
       uint64_t c[K];
 #pragma unroll
       for (int i = 0; i < K; ++i) c[i] = lane + 64 * i < C ? cand[lane + 64 * i] : 0;
-      const uint64_t bound = nth_bound<K>(c, n);
+      const uint64_t bound = nth_bound<K, sizeof(T) == 2 ? 16 : 0>(c, n, V);
       __builtin_amdgcn_wave_barrier();
       int at = 0;
 #pragma unroll
       for (int i = 0; i < K; ++i) {
-        const bool in = c[i] >= bound;
+        const bool in = c[i] != 0 && c[i] >= bound;
         const uint64_t mask = __ballot(in);
         if (in) cand[at + __popcll(mask & below)] = c[i];
         at += __popcll(mask);
