@@ -110,6 +110,23 @@ def test_values_and_gradient(R, V, top, mask, dt, device):
 
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('mask', ['none', 'inf', 'lowest'])
+@pytest.mark.parametrize('R,V,top', [(1, 70001, 64), (6, 131072, 20), (3, 200003, 0), (128, 66000, 5), (2, 530000, 64)])
+def test_few_long_rows(R, V, top, mask, dt, device):
+    """at every alignment, and with fewer elements above -inf than threads"""
+    if device == 'cpu' and R * V > 500000:
+        pytest.skip('the CPU form has one way for every size')
+    x, ids, g = _case(R, V, dt, mask, R + V, device)
+    grad = torch.randn(R, 2 + top, generator=g).to(device)
+    r = K.token_logprob(x, ids, top)
+    _check(x, ids, top, dt, r, K.token_logprob_backward(x, ids, r, grad), grad)
+    near = x.masked_fill(torch.arange(V, device=device) >= 40, -INF)
+    ids = torch.where(ids >= 0, ids % 40, ids)
+    _check(near, ids, min(top, 40), dt, K.token_logprob(near, ids, min(top, 40)))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
 def test_strided_rows_and_leading_dimensions(dt, device):
     """rows of a padded buffer at every alignment; [batch, position, V]; a transposed batch"""
     for off, V, pitch in ((0, 100, 104), (1, 999, 1003), (3, 30, 37), (5, 777, 778)):
