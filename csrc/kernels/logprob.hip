@@ -54,8 +54,6 @@ __device__ __forceinline__ Lse lse_join(Lse a, int G) {
   return r;
 }
 
-typedef unsigned Raw __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ void unpack(const Raw& q, float (&v)[4]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(q[k]);
@@ -503,10 +501,14 @@ __global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const 
 }
 
 // A block takes kBwdGranules granules of a row, the last row first: the logits that the forward
-// pass read last are still in the last-level cache.
-constexpr int kBwdThreads = 256, kBwdU = 4, kBwdGranules = kBwdThreads * kBwdU * 2;
+// pass read last are still in the last-level cache.  Bound by memory: 5.9 TB/s at 8192 x 30522.
+//   ST_PAST: the gradient goes past that cache (both passes 282 -> 249 us at 8192 x 30522 bf16, for
+//            the next forward pass reads at 5.6 instead of 4 TB/s; 777 x 50021 fp32 89 -> 65 us).
+//   LD_PAST: the logits too, where most of them cannot be there (this pass 354 -> 322 us at 4096 x
+//            131072 bf16, 1 GB; at 8192 x 30522, half of that, 166 -> 176).
+constexpr int kBwdThreads = 256, kBwdU = 4, kBwdGranules = kBwdThreads * kBwdU;
 
-template <typename T>
+template <typename T, bool LD_PAST, bool ST_PAST>
 __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __restrict__ logits, int64_t stride,
                                                                    const int64_t* __restrict__ ids, int64_t R, int V,
                                                                    int n, int64_t ignored, int chunks,
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
       for (int k = 0; k < VE; ++k) v[k] = slope(v[k]);
     }
     if (j >= w.f0 && j < w.f1) {
-      store_vec<T>(d + e0, v);
+      store_raw<ST_PAST>(d + e0, pack_raw(v));
     } else {
 #pragma unroll
       for (int k = 0; k < VE; ++k)
@@ -566,14 +568,14 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
     for (; j + (U - 1) * NT < a1; j += U * NT) {
       Raw q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = r.raw(j + u * NT);
+      for (int u = 0; u < U; ++u) q[u] = load_raw<LD_PAST>(r.x - r.off + (int64_t)(j + u * NT) * VE);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float v[VE];
         unpack(q[u], v);
 #pragma unroll
         for (int k = 0; k < VE; ++k) v[k] = slope(v[k]);
-        store_vec<T>(d + (int64_t)(j + u * NT) * VE - w.off, v);
+        store_raw<ST_PAST>(d + (int64_t)(j + u * NT) * VE - w.off, pack_raw(v));
       }
     }
     for (; j < a1; j += NT) take(j);
@@ -646,10 +648,13 @@ HETU_API int hetu_token_logprob_bwd(const void* logits, int64_t stride, const in
   const int64_t chunks = ((int64_t)V + 2 * VE - 2 + (int64_t)VE * kBwdGranules - 1) / ((int64_t)VE * kBwdGranules);
   if (V < 1 || n < 0 || n > kMaxTop || n > V || R > kMaxBlocks / chunks) return (int)hipErrorInvalidValue;
   const dim3 grid = many_blocks(R * chunks), block(kBwdThreads);
-  if (is_bf16)
-    hipLaunchKernelGGL(token_logprob_bwd_k<bf16>, grid, block, 0, st, (const bf16*)logits, stride, ids, R, V, n, ignored, (int)chunks, out, top, grad, (bf16*)dx);
-  else
-    hipLaunchKernelGGL(token_logprob_bwd_k<float>, grid, block, 0, st, (const float*)logits, stride, ids, R, V, n, ignored, (int)chunks, out, top, grad, (float*)dx);
+  const int64_t bytes = R * V * (is_bf16 ? 2 : 4);
+#define GO(T, LD, ST) hipLaunchKernelGGL((token_logprob_bwd_k<T, LD, ST>), grid, block, 0, st, (const T*)logits, stride, ids, \
+                                         R, V, n, ignored, (int)chunks, out, top, grad, (T*)dx)
+  if (bytes > 3 * kLastCacheBytes) { if (is_bf16) GO(bf16, true, true); else GO(float, true, true); }
+  else if (2 * bytes > kLastCacheBytes) { if (is_bf16) GO(bf16, false, true); else GO(float, false, true); }
+  else { if (is_bf16) GO(bf16, false, false); else GO(float, false, false); }
+#undef GO
   HETU_LAUNCH_CHECK();
   return 0;
 }

@@ -44,10 +44,10 @@ __device__ __forceinline__ void tokens_on(const void* valid, int kind, int64_t t
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool PAST>
 __device__ __forceinline__ void store_n(T* p, const float (&v)[V]) {
   if constexpr (V == 1) p[0] = from_f<T>(v[0]);
-  else store_vec<T>(p, v);
+  else store_raw<PAST>(p, pack_raw(v));
 }
 
 // A lane's elements of a row as they are in memory: converted when they are used, so that loads
@@ -55,8 +55,7 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[V]) {
 // hold the row's first elements again: they leave the maximum as it is, and are left out of sums.
 template <typename T, int V, int NJ, int G>
 struct RowRaw {
-  typedef unsigned Q4 __attribute__((ext_vector_type(4)));
-  Q4 q[V == 1 ? 1 : NJ];
+  Raw q[V == 1 ? 1 : NJ];
   T s[V == 1 ? NJ : 1];
   __device__ __forceinline__ void load(const T* x, int E, int lane) {
 #pragma unroll
@@ -64,14 +63,14 @@ struct RowRaw {
       int e = (j * G + lane) * V;
       e = e < E ? e : 0;
       if constexpr (V == 1) s[j] = x[e];
-      else q[j] = *reinterpret_cast<const Q4*>(x + e);
+      else q[j] = *reinterpret_cast<const Raw*>(x + e);
     }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if constexpr (V == 1) s[j] = from_f<T>(0.f);
-      else q[j] = Q4{0, 0, 0, 0};
+      else q[j] = Raw{0, 0, 0, 0};
     }
   }
   __device__ __forceinline__ void unpack(float (&p)[NJ * V]) const {
@@ -334,8 +333,9 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_k(const float* __re
   }
 }
 
-// U rows a group at a time
-template <typename T, int V, int NJ, int G>
+// U rows a group at a time; PAST: the gradient goes past the last-level cache, in whole 16 bytes
+// (262144 x 256 bf16: the next call's partial sums 45 -> 37 us; single elements would take twice as long)
+template <typename T, int V, int NJ, int G, bool PAST>
 __global__ void __launch_bounds__(kBlThreads) balance_bwd_k(const T* __restrict__ x, int64_t stride, int64_t T_, int E,
                                                             const float* __restrict__ weight,
                                                             const float* __restrict__ g, const void* valid, int kind,
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kBlThreads) balance_bwd_k(const T* __restrict_
           float v[V];
 #pragma unroll
           for (int q = 0; q < V; ++q) v[q] = on[u] ? c * p[u][j * V + q] * (w[j * V + q] - dot[u]) : 0.f;
-          store_n<T, V>(dx + tu * (int64_t)E + e, v);
+          store_n<T, V, PAST>(dx + tu * (int64_t)E + e, v);
         }
       }
     }
@@ -399,7 +399,8 @@ struct RowPlan { int V, G, NJ; };
 // V elements a load where rows and buffers allow 16-byte accesses, G lanes a row, NJ loads a lane.
 // The vector unit bounds these kernels (about 9 issue slots an element, 5 more for each exchange of
 // a reduction and 15 for a row, in every lane), so a lane takes up to 16 elements and G is what they
-// leave: 262144 x 256 bf16 with 16 lanes a row against 32: see the measurements at the launches.
+// leave (262144 x 256 bf16: partial sums 46 us with 16 lanes a row, 52 with 32; 100003 x 161 fp32: 18
+// us with 16 lanes, 30 with 64).
 static RowPlan plan_rows(int E, int64_t stride, const void* x, const void* y, int vec) {
   RowPlan r;
   r.V = (E % vec == 0 && stride % vec == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0) ? vec : 1;
@@ -508,10 +509,16 @@ HETU_API int hetu_moe_balance_bwd(const void* x, int64_t stride, int64_t T, int 
   // 8 blocks a CU loop over the rows, for each block reads the weights: 262144 x 256 bf16 57 us, with
   // 8192 blocks 75, with one for each of its rows 122
   const dim3 grid((unsigned)(want < 2048 ? want : 2048));
+  const bool past = 2 * T * E * (is_bf16 ? 2 : 4) >= kLastCacheBytes;
   const auto go = [&](auto zero, auto v, auto nj, auto g) {
     typedef decltype(zero) TT;
-    hipLaunchKernelGGL((balance_bwd_k<TT, decltype(v)::value, decltype(nj)::value, decltype(g)::value>), grid,
-                       dim3(kBlThreads), 0, st, (const TT*)x, stride, T, E, weight, grad, valid, kind, (TT*)dx);
+    constexpr int V = decltype(v)::value, NJ = decltype(nj)::value, G = decltype(g)::value;
+    if (V > 1 && past)
+      hipLaunchKernelGGL((balance_bwd_k<TT, V, NJ, G, (V > 1)>), grid, dim3(kBlThreads), 0, st, (const TT*)x, stride, T,
+                         E, weight, grad, valid, kind, (TT*)dx);
+    else
+      hipLaunchKernelGGL((balance_bwd_k<TT, V, NJ, G, false>), grid, dim3(kBlThreads), 0, st, (const TT*)x, stride, T, E,
+                         weight, grad, valid, kind, (TT*)dx);
   };
   if (is_bf16) with_plan<8>(r, [&](auto v, auto nj, auto g) { go(bf16(), v, nj, g); });
   else with_plan<4>(r, [&](auto v, auto nj, auto g) { go(0.f, v, nj, g); });

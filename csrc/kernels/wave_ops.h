@@ -7,6 +7,38 @@
 
 namespace hetu {
 
+// ---- 16-byte accesses that leave the last-level cache alone -------------------------------------
+// What a kernel writes stays in that cache (256 MB) as dirty lines, which the next kernel's reads
+// have to push out.  Where a result cannot be found there anyway, for it and its input are larger than
+// the cache, it goes past it.  (Known at compile time: a branch between the two kinds is merged into
+// one plain access.)
+constexpr int64_t kLastCacheBytes = 256ll << 20;
+typedef unsigned Raw __attribute__((ext_vector_type(4)));
+
+template <bool PAST>
+__device__ __forceinline__ Raw load_raw(const void* p) {
+  const Raw* q = reinterpret_cast<const Raw*>(p);
+  if constexpr (PAST) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+template <bool PAST>
+__device__ __forceinline__ void store_raw(void* p, const Raw& v) {
+  Raw* q = reinterpret_cast<Raw*>(p);
+  if constexpr (PAST) __builtin_nontemporal_store(v, q);
+  else *q = v;
+}
+__device__ __forceinline__ Raw pack_raw(const float (&v)[4]) {
+  return Raw{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+__device__ __forceinline__ Raw pack_raw(const float (&v)[8]) {
+  Raw r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (unsigned)f_to_bf16_bits(v[2 * i]) | ((unsigned)f_to_bf16_bits(v[2 * i + 1]) << 16);
+  return r;
+}
+
+// ---- reductions -------------------------------------------------------------------------------
+
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {
   return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
