@@ -579,8 +579,10 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
       }
     }
     for (; j < a1; j += NT) take(j);
-    if (tid == 0 && chunk == 0 && w.has_head()) take(0);
-    if (tid == NT - 1 && chunk == chunks - 1 && w.has_tail()) take(w.ng - 1);
+    // (the tail to the chunk that holds it, whose block writes the tokens below too: the last chunk may
+    // be empty)
+    if (tid == 0 && j0 == 0 && w.has_head()) take(0);
+    if (tid == NT - 1 && w.ng - 1 >= j0 && w.ng - 1 < j1 && w.has_tail()) take(w.ng - 1);
   } else {         // rows of another alignment than the gradient's
     const int e0 = j0 * VE - w.off, e1 = j1 * VE - w.off;
     for (int e = (e0 < 0 ? 0 : e0) + tid; e < (e1 < V ? e1 : V); e += NT) d[e] = from_f<T>(slope(to_f(r.x[e])));

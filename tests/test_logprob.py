@@ -174,6 +174,24 @@ def test_ties_and_adversarial_orders(kind, device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('V', [4089, 4093, 4095, 4097, 8177, 8185, 8189, 8191, 8193, 16377])
+def test_tokens_at_the_ends_of_a_row(V, dt, device):
+    """the first and last tokens, given and among the alternatives, where a row ends near a block's share
+    of it, at every alignment: each gets its own terms once"""
+    wide, _, g = _case(33, V + 9, dt, 'none', V, device)
+    wide[:, :] = wide * 0.1
+    for off in range(9):
+        x = wide[:, off:off + V]
+        for i in (0, V - 2, V - 1):
+            x[:, i] = 9.0
+        ids = torch.tensor([0, V - 1, V // 2] * 11, device=device)
+        grad = 1000.0 * torch.randn(33, 5, generator=g).to(device)
+        r = K.token_logprob(x, ids, 3)
+        _check(x, ids, 3, dt, r, K.token_logprob_backward(x, ids, r, grad), grad)
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_rows_that_are_not_read(device):
     """ignored and out-of-range tokens: NaN and infinities in their rows reach nothing"""
     V = 500
