@@ -501,8 +501,8 @@ __global__ void __launch_bounds__(kShortWaves * 64) token_logprob_short_k(const 
 }
 
 // A block takes kBwdGranules granules of a row, the last row first: the logits that the forward
-// pass read last are still in the last-level cache.  Bound by memory: 5.9 TB/s at 8192 x 30522.
-//   ST_PAST: the gradient goes past that cache (both passes 282 -> 249 us at 8192 x 30522 bf16, for
+// pass read last are still in the last-level cache.  Bound by memory: 164 us at 8192 x 30522 bf16, 6.1 TB/s.
+//   ST_PAST: the gradient goes past that cache (both passes 282 -> 242 us at 8192 x 30522 bf16, for
 //            the next forward pass reads at 5.6 instead of 4 TB/s; 777 x 50021 fp32 89 -> 65 us).
 //   LD_PAST: the logits too, where most of them cannot be there (this pass 354 -> 322 us at 4096 x
 //            131072 bf16, 1 GB; at 8192 x 30522, half of that, 166 -> 176).
@@ -615,8 +615,9 @@ static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, i
                                        (const T*)logits, stride, ids, R, V, n, ignored, out, top)
   const int64_t bytes = (int64_t)V * sizeof(T);
   // 1024 threads for long rows that are few, or that have alternatives to find (a thread's elements are
-  // read again: 1000 x 131072 top 20 63 us, with 256 threads 71); 256 threads else (8192 x 30522 117
-  // us, with 128 130, with 512 124); a wave for rows that it holds in registers
+  // read again: 1000 x 131072 top 20 57 us, with 256 threads 71 against 63 then); 256 threads else (8192
+  // x 30522: 117 us, with 128 130, with 512 124, all before the gradient went past the cache, 81 since);
+  // a wave for rows that it holds in registers (16384 x 2000 bf16 top 64: 64 us)
   if (bytes <= kShortBytes) {
     const dim3 grid = many_blocks((R + kShortWaves - 1) / kShortWaves), block(64 * kShortWaves);
     if (n) hipLaunchKernelGGL((token_logprob_short_k<T, true>), grid, block, 0, st, (const T*)logits, stride, ids, R, V, n, ignored, out, top);

@@ -416,7 +416,8 @@ static RowPlan plan_rows(int E, int64_t stride, const void* x, const void* y, in
 using namespace hetu;
 
 // Rows a block of the partial sums takes: as many blocks as keep the chip's waves busy (2 blocks of 8
-// waves a CU; 1024 blocks gain the partial sums nothing and cost the join 2 us), but at least 2 rows a group of lanes, for each block costs E partial sums.
+// waves a CU; 1024 blocks gain the partial sums nothing and cost the join 2 us), but at least 2 rows a
+// group of lanes, for each block costs E partial sums.
 constexpr int kMaxParts = 512;
 static int64_t balance_rows(int64_t T, int G) {
   const int64_t groups = kPartThreads / G;
