@@ -260,6 +260,12 @@ __attribute__((amdgpu_num_sgpr(80))) __global__ void __launch_bounds__(NT) token
   if (tid == 0 && r.has_head()) {
     float v[1][VE];
     r.load(0, v[0]);
+    if (TOP) {                        // the row's first elements, taken last: where they tie, they are the sample
+      float vm = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) vm = fmaxf(vm, v[0][k]);
+      if (vm >= a.m) best = 0;
+    }
     lse_take<1, VE, TOP>(a, best, v, 0, NT);
   }
   if (tid == NT - 1 && r.has_tail()) {

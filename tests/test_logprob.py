@@ -347,3 +347,31 @@ def test_op_without_alternatives(device):
     r = K.token_logprob(x, ids)
     _check(x, ids, 0, torch.float32, r, torch.from_numpy(d), grad)
     np.testing.assert_allclose(lp, r.logp.numpy(), rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dt,V', [(torch.float32, 4097), (torch.float32, 9001), (torch.bfloat16, 9001), (torch.bfloat16, 20011)])
+def test_ties_with_the_first_elements_of_an_unaligned_row(dt, V, device):
+    """a row's first elements, up to its first 16-byte border, are taken apart from the rest: where they tie with
+    later ones, the lowest token still wins, at every alignment and for both sizes of a block"""
+    n = 16 // torch.empty((), dtype=dt).element_size()
+    threads = 1024 if V * (16 // n) >= 32768 else 256
+    g = torch.Generator().manual_seed(V)
+    for off in range(1, n):
+        wide = torch.full((4, -(-(V + off) // n) * n), -3.0)
+        for row, head in enumerate((0, n - off - 1, 0, 0)):
+            # the first elements, a thread far behind, and the first threads' second share alone
+            ties = [off + head, n * 101 + 3, n * (1 + threads), n * (2 + threads), n * (3 + threads), n * (4 + threads)]
+            wide[row, ties[:3] if row < 2 else ties] = 2.0
+            if row == 3:
+                wide[row, 5 * n::7] = 2.0
+        x = wide.to(dt).to(device)[:, off:off + V]
+        ids = torch.zeros(4, dtype=torch.int64, device=device)
+        for top in (1, 2, 3, 20, 40):
+            _check(x, ids, top, dt, K.token_logprob(x, ids, top))
+        whole = torch.randint(0, 7, (40, wide.shape[1]), generator=g).float().to(dt).to(device)[:, off:off + V]
+        whole[:, 0] = torch.where(torch.arange(40, device=device) % 2 == 0, 6.0, 0.0).to(dt)
+        whole[::2, 5:whole.shape[1] // 2] = 1.0
+        ids = torch.zeros(40, dtype=torch.int64, device=device)
+        for top in (1, 20, 64):
+            _check(whole, ids, top, dt, K.token_logprob(whole, ids, top))
