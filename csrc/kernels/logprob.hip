@@ -590,8 +590,12 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_k(const T* __re
     if (tid == 0 && j0 == 0 && w.has_head()) take(0);
     if (tid == NT - 1 && w.ng - 1 >= j0 && w.ng - 1 < j1 && w.has_tail()) take(w.ng - 1);
   } else {         // rows of another alignment than the gradient's
-    const int e0 = j0 * VE - w.off, e1 = j1 * VE - w.off;
-    for (int e = (e0 < 0 ? 0 : e0) + tid; e < (e1 < V ? e1 : V); e += NT) d[e] = from_f<T>(slope(to_f(r.x[e])));
+    const int a0 = j0 * VE - w.off, b0 = a0 < 0 ? 0 : a0;                       // (b0 + NT may pass 32 bits, the count not)
+    const int64_t a1 = (int64_t)j1 * VE - w.off;
+    const int count = (int)(a1 < V ? a1 : V) - b0;
+    const T* xs = r.x + b0;
+    T* ds = d + b0;
+    for (int e = tid; e < count; e += NT) ds[e] = from_f<T>(slope(to_f(xs[e])));
   }
   if (dead) return;
   // this chunk's part of the given token and the alternatives once more, each with its own terms:

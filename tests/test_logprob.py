@@ -375,3 +375,26 @@ def test_ties_with_the_first_elements_of_an_unaligned_row(dt, V, device):
         ids = torch.zeros(40, dtype=torch.int64, device=device)
         for top in (1, 20, 64):
             _check(whole, ids, top, dt, K.token_logprob(whole, ids, top))
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_longest_row_at_another_alignment():
+    """2^31 - 65 logits of a row that starts one element off the gradient's alignment: the last elements'
+    numbers plus a block's threads pass 31 bits"""
+    V = 2 ** 31 - 65
+    x = torch.zeros(V + 1, dtype=torch.bfloat16, device='cuda')[1:]
+    x[V - 3] = 20.0
+    ids = torch.tensor([V - 1], device='cuda')
+    r = K.token_logprob(x[None], ids)
+    # S = (V - 1) e^-20 + 1: a thread adds 2^21 terms one after another, of which each sum of 32 is one
+    lse = 20.0 + math.log1p((V - 1) * math.exp(-20.0))
+    slack = U * (2 ** 21 / 32 + 200)
+    assert abs(float(r.logp[0]) + lse) <= slack + 4 * U * lse
+    d = K.token_logprob_backward(x[None], ids, r, torch.tensor([[1.0, 0.0]], device='cuda'))[0]
+    p = math.exp(-lse)
+    step = 2.0 ** -8 + 2 * slack + 40 * U
+    for a, b in ((0, 3000), (V // 2, V // 2 + 3000), (V - 3000, V - 3)):
+        assert bool(((d[a:b].double() + p).abs() <= step * p).all())
+    assert bool(((d[3000:V - 3000:4099].double() + p).abs() <= step * p).all())
+    want = torch.tensor([-math.exp(20.0) * p, -p, 1.0 - p], dtype=torch.float64, device='cuda')
+    assert bool(((d[V - 3:].double() - want).abs() <= step * want.abs()).all())
