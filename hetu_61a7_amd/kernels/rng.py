@@ -110,9 +110,17 @@ def next_seed(key, on_gpu=True):
 
 
 def fixed_seed(key, place=0):
-    """a seed of op ``key`` that is the same in every step: for kernels that take the step number
-    from elsewhere"""
-    return _mix(_BASE[0] ^ _mix((int(key) << 20) ^ 0xF1) ^ _mix(int(place)))
+    """a seed of ``key`` and ``place`` alone, the same in every step, process and run: for kernels that
+    take the step number from elsewhere"""
+    return _mix(_mix(int(key) ^ 0xF1) ^ _mix(int(place)))
+
+
+def key_of(numbers):
+    """a key for ``fixed_seed`` from a sequence of whole numbers"""
+    k = 0
+    for n in numbers:
+        k = _mix(k ^ int(n))
+    return k
 
 
 # ---- random fills / channel dropout ---------------------------------------------------------

@@ -185,8 +185,9 @@ class AdamWOptimizer(AdamOptimizer):
 
     def _update8(self, flat, param, grad, own, shadow, step, dyn):
         """one adamw8 launch over flat elements ``own`` of the state.  The rounding's seed follows
-        from the run's seed, the place and the step number alone: the same on every replica, in a
-        replayed step, and after a resume."""
+        from the sizes of the flat buffer's parameters (``rng_key``), the place and the step number
+        alone: the same on every replica, in a replayed step, and after a resume, whatever else a
+        process built or ran."""
         from .kernels import rng
         seed = rng.fixed_seed(flat.rng_key, own.start)
         if dyn is None:
@@ -269,6 +270,8 @@ class FlatGroup(object):
         self.s1_scale = self.s2_scale = None
         self.rng_key = 0
         if state_bits == 8:
+            from .kernels import rng
+            self.rng_key = rng.key_of(self.offsets[p][1] for p in params)
             self.s1, self.s2, self.s1_scale, self.s2_scale = KO.adamw8_state(ns, dev)
         else:
             self.s1 = _filled((ns,), state_init[0], dev) if n_states >= 1 else None
@@ -416,7 +419,6 @@ class OptimizerOp(Op):
         self.flat = FlatGroup(dense, values, opt.n_states, getattr(opt, 'state_init', (0.0, 0.0)),
                               shadow=amp, device=self.ctx.torch_device if self.ctx else None,
                               pad_to=pad_to, state_numel=state_numel, state_bits=opt.state_bits)
-        self.flat.rng_key = self.id
         # ops that can write their gradient straight into the flat buffer get its view
         grad_of = {pp: g for pp, g in zip(self.param_of_input, self.inputs)}
         for p in dense:

@@ -307,3 +307,33 @@ def test_replayed_steps_equal_eager_ones():
         assert train.step == 8
     for a, b in zip(*runs):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_resume_rounds_alike_in_another_process(tmp_path, device):
+    """other nodes and other executors, of other seeds, built before and between: the steps after a resume are
+    those of the run that was not interrupted, bit by bit"""
+    ctx = ht.cpu(0) if device == 'cpu' else ht.gpu(0)
+
+    def make(seed):
+        rng = np.random.RandomState(1)
+        x, y_, loss, train = _net(8, rng)
+        return ht.Executor({'train': [loss, train]}, ctx=ctx, seed=seed), x, y_, train
+
+    def steps(ex, x, y_, a, b):
+        for i in range(a, b):
+            ex.run('train', feed_dict=_feed(np.random.RandomState(100 + i), x, y_))
+
+    ex, x, y_, train = make(3)
+    steps(ex, x, y_, 0, 3)
+    ex.save(str(tmp_path), save_optimizer=True)
+    steps(ex, x, y_, 3, 8)
+    ht.Variable(name='unused', value=np.zeros(2, np.float32))
+    ex2, x2, y2, train2 = make(11)
+    ex2.load(str(tmp_path))
+    steps(ex2, x2, y2, 3, 5)
+    w = ht.Variable(name='w', value=np.ones(3, np.float32))
+    ht.Executor({'eval': [ht.reduce_mean_op(w, [0])]}, ctx=ctx, seed=99)
+    steps(ex2, x2, y2, 5, 8)
+    for k in ('param', 's1', 's2', 's1_scale', 's2_scale'):
+        assert torch.equal(getattr(train.flat, k).view(torch.uint8), getattr(train2.flat, k).view(torch.uint8)), k

@@ -96,6 +96,44 @@ def test_two_ranks(tmp_path, zero):
         assert near.mean() > 0.98, k          # (gradients of nearly nothing may differ more)
 
 
+def _other_process_worker(rank, port, zero, q):
+    """replicas whose processes differ in all but the model: nodes built before, an executor of another
+    seed built later, the executor's own seed"""
+    os.environ.update(RANK=str(rank), WORLD_SIZE='2', LOCAL_RANK=str(rank), MASTER_ADDR='127.0.0.1',
+                      MASTER_PORT=str(port), HETU_USE_CONFIG='0')
+    import hetu_61a7_amd as ht
+    if rank == 0:
+        for i in range(3):
+            ht.Variable(name='unused%d' % i, value=np.zeros(2, np.float32))
+    executor = ht.Executor
+    ht.Executor = lambda *a, **k: executor(*a, **dict(k, seed=5 + rank))
+    ex, x, y_, train = _make(8, True, zero)
+    ht.Executor = executor
+    part = slice(rank * 8, rank * 8 + 8)
+    _run(ex, x, y_, [0], part)
+    if rank == 0:
+        w = ht.Variable(name='w', value=np.ones(3, np.float32))
+        ht.Executor({'eval': [ht.reduce_mean_op(w, [0])]}, ctx=ht.cpu(0), seed=99)
+    q.put((rank, _run(ex, x, y_, [1, 2, 3, 4], part)))
+    from hetu_61a7_amd.parallel import comm
+    comm.destroy()
+
+
+@pytest.mark.parametrize('zero', [0, 1])
+def test_replicas_of_unlike_processes_stay_equal(zero):
+    ctx = mp.get_context('spawn')
+    q, port = ctx.Queue(), _free_port()
+    procs = [ctx.Process(target=_other_process_worker, args=(r, port, zero, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    for k in got[0]:
+        np.testing.assert_array_equal(got[0][k], got[1][k])
+
+
 def test_whole_moments_load_into_shards_of_another_layout(tmp_path):
     """32-bit moments of a buffer aligned to 8 elements are found by name in a buffer aligned to 256"""
     from hetu_61a7_amd.utils.checkpoint import _relaid, _read
