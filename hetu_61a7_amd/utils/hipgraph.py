@@ -80,6 +80,31 @@ def _close_all():
 atexit.register(_close_all)
 
 
+class _StepScalars(object):
+    """pinned rows that the steps' scalars are copied from.  The host may be many steps ahead of the
+    device: a row is written again only after the copy out of it has run, which an event for each
+    half of the rows tells."""
+    HALF = 32
+
+    def __init__(self, n):
+        self.rows = _NA.zeros(2 * self.HALF, n, dtype=torch.float32).pin_memory()
+        self.at, self.copied = 0, [None, None]
+
+    def copy_to(self, dst, values):
+        from ..runtime import DeviceEvent
+        half, place = divmod(self.at, self.HALF)
+        if place == 0 and self.copied[half] is not None:
+            self.copied[half].synchronize()
+        row = self.rows[self.at]
+        row.copy_(torch.tensor(values, dtype=torch.float32))
+        dst.copy_(row, non_blocking=True)
+        if place == self.HALF - 1:
+            if self.copied[half] is None:
+                self.copied[half] = DeviceEvent()
+            self.copied[half].record()
+        self.at = (self.at + 1) % (2 * self.HALF)
+
+
 class GraphRunner(object):
     def __init__(self, sub, warmup=3):
         _RUNNERS.add(self)
@@ -121,17 +146,12 @@ class GraphRunner(object):
             if getattr(op, 'dyn', None) is None:
                 # lr, beta1^t, beta2^t, gradient scale, step, 1 - beta1^t, 1 - beta2^t
                 op.dyn = _NA.zeros(7, dtype=torch.float32, device=self.sub.config.device)
-                op.dyn_host = _NA.zeros(7, dtype=torch.float32).pin_memory()
+                op.dyn_host = _StepScalars(7)
             step = op.step + 1
             h = opt.hyper(step)
-            op.dyn_host[0] = h.get('lr', 0.0)
-            op.dyn_host[1] = h.get('beta1t', 1.0)
-            op.dyn_host[2] = h.get('beta2t', 1.0)
-            op.dyn_host[3] = op.flat.gscale if op.flat is not None else 1.0
-            op.dyn_host[4] = step
-            op.dyn_host[5] = 1.0 - h.get('beta1t', 1.0)
-            op.dyn_host[6] = 1.0 - h.get('beta2t', 1.0)
-            op.dyn.copy_(op.dyn_host, non_blocking=True)
+            b1t, b2t = h.get('beta1t', 1.0), h.get('beta2t', 1.0)
+            op.dyn_host.copy_to(op.dyn, [h.get('lr', 0.0), b1t, b2t, op.flat.gscale if op.flat is not None else 1.0,
+                                         step, 1.0 - b1t, 1.0 - b2t])
 
     def run(self, feed_dict, convert):
         sub = self.sub

@@ -337,3 +337,33 @@ def test_resume_rounds_alike_in_another_process(tmp_path, device):
     steps(ex2, x2, y2, 5, 8)
     for k in ('param', 's1', 's2', 's1_scale', 's2_scale'):
         assert torch.equal(getattr(train.flat, k).view(torch.uint8), getattr(train2.flat, k).view(torch.uint8)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [8, 32])
+def test_steps_replayed_without_waiting_take_their_own_scalars(bits):
+    """the host may be many steps ahead of the device: each replayed step has the rates, bias corrections and
+    rounding seed of its own number"""
+    runs = []
+    for graph in (False, True):
+        rng = np.random.RandomState(2)
+        rate = ht.lr.ExponentialScheduler(0.01, 0.95)
+        x, y_, loss, train = _net(bits, rng, lr=rate)
+        ex = ht.Executor({'train': [loss, train]}, ctx=ht.gpu(0), seed=3, use_hipgraph=graph)
+        feed = {n: torch.from_numpy(v).cuda() for n, v in _feed(rng, x, y_).items()}
+        busy = torch.ones(4096, 4096, device='cuda')
+        for i in range(5 + 150):
+            if i == 5:                             # captured by now: the device gets work for some 50 ms
+                torch.cuda.synchronize()
+                for _ in range(60):
+                    busy = torch.mm(busy, busy) * 1e-4
+            ex.run('train', feed_dict=feed)
+            rate.step()
+            if not graph:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        f = train.flat
+        assert train.step == 155
+        runs.append([t.clone().view(torch.uint8) for t in (f.param, f.s1, f.s2)])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
