@@ -27,7 +27,7 @@ struct Adam8Args {
   // 32 bits is off by 1e-5 of itself)
   float lr, beta1, beta2, omb1, omb2, omb1t, omb2t, eps, wd, gscale;
   // {lr, -, -, gscale, step, omb1t, omb2t} on the device, or null: a captured step's own.  The
-  // step number moves the seed, as the caller moves it without dyn.
+  // step number, modulo the 2^24 that fp32 holds, moves the seed, as the caller moves it without dyn.
   const float* dyn;
   uint64_t seed;
 };
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256) adamw8_k(float* __restrict__ p, const flo
   uint64_t key = a.seed;
   if (a.dyn) {
     lr = a.dyn[0]; gsc = a.dyn[3]; c1 = a.dyn[5]; c2 = a.dyn[6];
-    key += (uint64_t)a.dyn[4] * kRngMix;
+    key += ((uint64_t)a.dyn[4] & 0xFFFFFFu) * kRngMix;
   }
   const float r1 = 1.f / c1, r2 = 1.f / c2;
   const unsigned seed = (unsigned)key ^ (unsigned)(key >> 32);

@@ -87,9 +87,14 @@ def _i64(seed):
     return seed - (1 << 64) if seed >> 63 else seed
 
 
+# step numbers that fp32 holds one by one: the seeds start again beyond them, for a captured step has
+# its number as fp32
+STEP_SEEDS = 1 << 24
+
+
 def step_seed(seed, step):
-    """the rounding seed of one step"""
-    return (int(seed) + int(step) * 0x9E3779B97F4A7C15) & _M64
+    """the rounding seed of one step (of step modulo 2^24)"""
+    return (int(seed) + int(step) % STEP_SEEDS * 0x9E3779B97F4A7C15) & _M64
 
 
 def adamw8_state(n, device):
@@ -151,8 +156,8 @@ def adamw8(p, g, m, v, m_scale, v_scale, shadow=None, *, lr, beta1=0.9, beta2=0.
     The update takes the fresh moments in 32 bits; what is stored of them is rounded at random,
     by bits that a hash of ``seed`` (64 bits) and the element's index gives: another seed every
     step.  ``dyn``: fp32 {lr, beta1t, beta2t, gscale, step, 1 - beta1t, 1 - beta2t} on the device
-    instead of the arguments, for a captured step; the seed is then moved by ``step`` as
-    ``step_seed`` moves it.
+    instead of the arguments, for a captured step; the seed is then moved by ``step`` (modulo
+    ``STEP_SEEDS``) as ``step_seed`` moves it.
     ``shadow`` (bf16, the weights' copy) is written too.  A block of 256 shares one scale: where
     several tensors share the buffer, start each at a multiple of 256.  ``eps`` is at least 1e-12."""
     n = p.numel()

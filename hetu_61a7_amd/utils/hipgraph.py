@@ -141,17 +141,18 @@ class GraphRunner(object):
         return vals
 
     def _update_dyn(self):
+        from ..kernels.optim import STEP_SEEDS
         for op in self.sub.opt_ops:
             opt = op.optimizer
             if getattr(op, 'dyn', None) is None:
-                # lr, beta1^t, beta2^t, gradient scale, step, 1 - beta1^t, 1 - beta2^t
+                # lr, beta1^t, beta2^t, gradient scale, step number for the rounding's seed, 1 - beta1^t, 1 - beta2^t
                 op.dyn = _NA.zeros(7, dtype=torch.float32, device=self.sub.config.device)
                 op.dyn_host = _StepScalars(7)
             step = op.step + 1
             h = opt.hyper(step)
             b1t, b2t = h.get('beta1t', 1.0), h.get('beta2t', 1.0)
             op.dyn_host.copy_to(op.dyn, [h.get('lr', 0.0), b1t, b2t, op.flat.gscale if op.flat is not None else 1.0,
-                                         step, 1.0 - b1t, 1.0 - b2t])
+                                         step % STEP_SEEDS, 1.0 - b1t, 1.0 - b2t])
 
     def run(self, feed_dict, convert):
         sub = self.sub

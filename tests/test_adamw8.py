@@ -367,3 +367,33 @@ def test_steps_replayed_without_waiting_take_their_own_scalars(bits):
         runs.append([t.clone().view(torch.uint8) for t in (f.param, f.s1, f.s2)])
     for a, b in zip(*runs):
         assert torch.equal(a, b)
+
+
+def test_seeds_of_neighbouring_steps_differ_beyond_what_fp32_counts():
+    """a captured step has its number as fp32: steps 2^24 and 2^24 + 1 have other seeds all the same, and the
+    seeds of a step whose number is an argument"""
+    for step in (5, (1 << 24) - 1, 1 << 24, (1 << 24) + 1, (1 << 25) + 3):
+        assert KO.step_seed(9, step) != KO.step_seed(9, step + 1)
+        a, b = _inputs(600, 3, 'cpu'), _inputs(600, 3, 'cpu')
+        KO.adamw8(*a, seed=KO.step_seed(9, step), **H)
+        dyn = torch.tensor([H['lr'], 0.0, 0.0, 1.0, step % KO.STEP_SEEDS, 1 - H['beta1t'], 1 - H['beta2t']], dtype=torch.float32)
+        KO.adamw8(*b, seed=9, dyn=dyn, **dict(H, lr=0.0))
+        assert torch.equal(a[2].view(torch.uint8), b[2].view(torch.uint8))
+        assert torch.equal(a[3].view(torch.uint8), b[3].view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_replayed_steps_equal_eager_ones_beyond_what_fp32_counts():
+    runs = []
+    for graph in (False, True):
+        rng = np.random.RandomState(2)
+        x, y_, loss, train = _net(8, rng)
+        ex = ht.Executor({'train': [loss, train]}, ctx=ht.gpu(0), seed=3, use_hipgraph=graph)
+        feed = _feed(rng, x, y_)
+        train.step = (1 << 24) - 6
+        for i in range(12):
+            ex.run('train', feed_dict=feed)
+            torch.cuda.synchronize()
+        runs.append([t.clone().view(torch.uint8) for t in (train.flat.param, train.flat.s1, train.flat.s2)])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
