@@ -253,6 +253,30 @@ def _ext_state(ex, zero_rank):
     return ext
 
 
+def _check_shard(op, d, shard, i):
+    """a ZeRO-1 shard is taken as it lies: refuse one whose elements lie elsewhere than this rank's (``d``:
+    its optimizer's record, with the parameters' places).  A shard of older form does not say which
+    ranges it owns: its parameters' places and its moments' width have to be the same then."""
+    fl = op.flat
+    bits = 8 if shard.get('s1_scale') is not None else 32
+    here = [(p.name, int(fl.offsets[p][0]), int(fl.offsets[p][1])) for p in fl.params]
+    same = True
+    if d.get('layout') is not None:
+        there = {name: (o, n) for name, o, n in d['layout']}
+        same = [(o, n) for _, o, n in d['layout']] == [(o, n) for _, o, n in here] and \
+            all(there.get(name, (o, n)) == (o, n) for name, o, n in here)
+    if shard.get('own') is not None:
+        same = same and [tuple(r) for r in shard['own']] == [tuple(b.own) for b in op.buckets]
+    else:
+        same = same and bits == fl.state_bits
+    same = same and all(shard.get(k) is None or np.size(shard[k]) == getattr(fl, k).numel()
+                        for k in ('s1', 's2') if getattr(fl, k) is not None)
+    if not same:
+        raise ValueError('optimizer %d: its ZeRO-1 shard was saved with %d-bit moments of another layout (here: %d-bit '
+                         'moments; parameters, bucket size and state_bits have to be those of the run that saved it, '
+                         'or it has to be saved without ZeRO-1)' % (i, bits, fl.state_bits))
+
+
 def _zero_shards(ex):
     out = []
     for op in _opt_ops(ex):
@@ -260,7 +284,7 @@ def _zero_shards(ex):
         if not getattr(op, 'zero', False) or fl is None:
             out.append(None)
             continue
-        out.append(dict(_moments(fl), nrank=op.comm.nrank, rank=op.comm.rank))
+        out.append(dict(_moments(fl), nrank=op.comm.nrank, rank=op.comm.rank, own=[tuple(b.own) for b in op.buckets]))
     return out
 
 
@@ -442,6 +466,8 @@ def load(ex, file_path, file_name='checkpoint.pkl', consider_splits=False):
             if src.get('nrank', op.comm.nrank) != op.comm.nrank:
                 raise ValueError('ZeRO checkpoint was written with %s ranks, resuming with %d'
                                  % (src.get('nrank'), op.comm.nrank))
+            if fl is not None and shards is not None and i < len(shards) and src is shards[i]:
+                _check_shard(op, d, src, i)
         if fl is not None:
             if src is d:
                 _load_flat_moments(fl, d, i)

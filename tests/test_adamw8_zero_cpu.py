@@ -146,3 +146,67 @@ def test_whole_moments_load_into_shards_of_another_layout(tmp_path):
     for p8, p in zip(t8.flat.params, train.flat.params):
         (o8, n, _), (o, _, _) = t8.flat.offsets[p8], train.flat.offsets[p]
         np.testing.assert_array_equal(full['s2'][o8:o8 + n], train.flat.s2[o:o + n].numpy())
+
+
+def _shard_worker(rank, port, path, q):
+    """saves shards of both widths and of another bucket size, and loads each into each"""
+    os.environ.update(RANK=str(rank), WORLD_SIZE='2', LOCAL_RANK=str(rank), MASTER_ADDR='127.0.0.1',
+                      MASTER_PORT=str(port), HETU_USE_CONFIG='0')
+    import hetu_61a7_amd as ht
+
+    def make(bits, sizes, bucket):
+        ws = [ht.Variable(name='w%d' % i, value=np.linspace(-1, 1 + i, n).astype(np.float32)) for i, n in enumerate(sizes)]
+        x = ht.Variable(name='x')
+        loss = ht.reduce_mean_op(x, [0])
+        for w in ws:
+            loss = loss + ht.reduce_mean_op(w * w, [0])
+        train = ht.optim.AdamWOptimizer(0.01, state_bits=bits).minimize(loss, var_list=ws)
+        ex = ht.Executor({'train': [loss, train]}, dist_strategy=ht.dist.DataParallel('allreduce'), zero=1,
+                         bucket_mb=bucket, seed=5)
+        return ex, x, train
+
+    got = {}
+    # (500, 500): the shards of both widths have 512 elements, the second parameter starts at 504 and 512
+    for sizes in ((500, 500), (200, 250), (2048, 1024)):
+        made = {}
+        for bits, bucket in ((32, 32), (8, 32), (8, 0.004)):
+            ex, x, train = made[bits, bucket] = make(bits, sizes, bucket)
+            for _ in range(3):
+                ex.run('train', feed_dict={x: np.ones(4, np.float32)})
+            ex.save('%s/%d_%d_%g' % (path, sizes[0], bits, bucket), save_optimizer=True)
+        for src in made:
+            for dst in made:
+                ex, x, train = make(dst[0], sizes, dst[1])
+                try:
+                    ex.load('%s/%d_%d_%g' % (path, sizes[0], src[0], src[1]))
+                    fl, old = train.flat, made[src][2].flat
+                    ok = all(torch.equal(getattr(fl, k).view(torch.uint8), getattr(old, k).view(torch.uint8))
+                             for k in ('s1', 's2')) if src[0] == dst[0] else 'converted'
+                    got[sizes, src, dst] = ok
+                except ValueError as e:
+                    got[sizes, src, dst] = 'refused' if 'ZeRO-1 shard' in str(e) else str(e)
+    q.put((rank, got))
+    from hetu_61a7_amd.parallel import comm
+    comm.destroy()
+
+
+def test_shards_of_another_layout_are_refused(tmp_path):
+    """a shard is a run of flat elements: one whose parameters start elsewhere (moments of the other width),
+    or whose buckets are split elsewhere, is refused, not loaded under other weights"""
+    ctx = mp.get_context('spawn')
+    q, port = ctx.Queue(), _free_port()
+    procs = [ctx.Process(target=_shard_worker, args=(r, port, str(tmp_path), q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    assert len(got[0]) == 27
+    for r in (0, 1):
+        for (sizes, src, dst), how in got[r].items():
+            # sizes of whole blocks lie alike in both widths, and one bucket splits them alike
+            alike = src == dst or (sizes == (2048, 1024) and src[1] == dst[1])
+            one_bucket = sizes[0] < 1000 and src[0] == dst[0]
+            want = True if src[0] == dst[0] else 'converted'
+            assert how == (want if alike or one_bucket else 'refused'), (r, sizes, src, dst, how)
