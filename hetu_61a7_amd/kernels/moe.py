@@ -173,6 +173,8 @@ def balance_loss(logits, indices, num_experts, valid=None):
     if indices.dim() < 1 or indices.shape[0] != T or T and indices.numel() % T or indices.device != x.device:
         raise ValueError('balance_loss: indices have to be [%d, k] on %s, got %s on %s'
                          % (T, x.device, tuple(indices.shape), indices.device))
+    if indices.is_floating_point() and indices.dtype not in (torch.float32, torch.float64):
+        raise ValueError('balance_loss: indices in %s, which does not hold every expert\'s number' % indices.dtype)
     idx = indices
     if idx.dim() != 2:
         idx = idx.reshape(T, -1) if idx.numel() else idx.reshape(T, 0)

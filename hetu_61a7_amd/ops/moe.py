@@ -546,6 +546,9 @@ class BalanceLossOp(Op):
         indices_s = list(indices_s) if isinstance(indices_s, (list, tuple)) else [indices_s]
         super().__init__(BalanceLossOp, [logits] + indices_s + ([valid] if valid is not None else []), ctx)
         self.k, self.num_experts, self.has_valid = len(indices_s), int(num_experts), valid is not None
+        from .loss import _label_feed
+        for n in indices_s:
+            _label_feed(n)          # expert ids: never cast to bf16 by a mixed-precision feed
 
     def compute(self, input_vals, output_val=None, stream_handle=None):
         from .nn import AuxResult

@@ -221,3 +221,29 @@ def test_mask_is_refused_by_other_gates():
     layer = ht.layers.MoELayer(ht.layers.KTop1Gate(8, 24, 4, k=2), [ht.layers.Expert(8, 8)], 24, 8)
     with pytest.raises(ValueError):
         layer(ht.Variable(name='x'), ht.Variable(name='m'))
+
+
+@pytest.mark.gpu
+def test_fed_choices_keep_their_experts_under_mixed_precision():
+    """choices fed as fp32 are labels: no cast to bf16, which holds whole numbers up to 256 alone"""
+    T, E = 1200, 600
+    rng = np.random.RandomState(2)
+    xv, iv = rng.randn(T, E).astype(np.float32), rng.randint(0, E, (T, 2))
+    X, I, V = ht.Variable(name='x', value=xv), ht.Variable(name='i', trainable=False), ht.Variable(name='v', trainable=False)
+    loss, counts = ht.balance_loss_op(X, I, E, V)
+    ex = ht.Executor({'train': [loss, counts]}, ctx=ht.gpu(0), mixed_precision='bf16')
+    on = np.arange(T) < T - 100
+    l, c = ex.run('train', feed_dict={I: iv.astype(np.float32), V: on.astype(np.float32)}, convert_to_numpy_ret_vals=True)
+    np.testing.assert_array_equal(c, np.bincount(iv[on].reshape(-1), minlength=E))
+
+
+def test_choices_in_types_that_skip_whole_numbers_are_refused():
+    x, idx, valid, g = _case(10, 8, 2, torch.float32, 'most', 4, 'cpu')
+    for dt in (torch.bfloat16, torch.float16):
+        with pytest.raises(ValueError):
+            K.balance_loss(x, idx.to(dt), 8)
+    for dt in (torch.float32, torch.float64, torch.int32):
+        assert torch.equal(K.balance_loss(x, idx.to(dt), 8).counts, K.balance_loss(x, idx, 8).counts)
+    I, V = ht.Variable(name='i', trainable=False), ht.Variable(name='v', trainable=False)
+    ht.balance_loss_op(ht.Variable(name='x'), I, 8, V)
+    assert I.keep_fp32                                # (what a feed under mixed precision goes by)
