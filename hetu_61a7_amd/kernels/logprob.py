@@ -137,6 +137,12 @@ def token_logprob_backward(logits, ids, fwd, grad, ignored_index=-1):
     if tuple(fwd.buffer.shape) != lead + (4 + top,) or grad.numel() != R * (2 + top) or grad.device != x.device:
         raise ValueError('token_logprob_backward: logits %s, forward of %s, gradient %s'
                          % (tuple(logits.shape), tuple(fwd.buffer.shape[:-1]), tuple(grad.shape)))
+    for t, shape, dt in ((fwd.buffer, lead + (4 + top,), torch.float32), (fwd.ids, lead + (top,), torch.int64)):
+        if t is None and not top:
+            continue
+        if t is None or tuple(t.shape) != shape or t.dtype != dt or t.device != x.device or not t.is_contiguous():
+            raise ValueError('token_logprob_backward: the forward result has to be whole and on %s: %s %s expected, got %s'
+                             % (x.device, dt, shape, t if t is None else (t.dtype, tuple(t.shape), t.device)))
     if grad.dtype != torch.float32 or not grad.is_contiguous():
         from .moe import _dc
         grad = _dc(grad, torch.float32)

@@ -215,6 +215,10 @@ def balance_loss_backward(logits, fwd, grad, valid=None):
     if fwd.experts != E or grad.numel() != 1 or grad.device != x.device:
         raise ValueError('balance_loss_backward: %d experts, weights of %d, a gradient of %s'
                          % (E, fwd.experts, tuple(grad.shape)))
+    b = fwd.buffer
+    if b.dtype != torch.int64 or b.numel() != E + E // 2 + 1 or b.device != x.device or not b.is_contiguous():
+        raise ValueError('balance_loss_backward: the forward result has to be whole and on %s, got %s %s on %s'
+                         % (x.device, b.dtype, tuple(b.shape), b.device))
     if native(x):
         check_device(x, 'balance_loss_backward')
         grad = _dc(grad, torch.float32)

@@ -247,3 +247,13 @@ def test_choices_in_types_that_skip_whole_numbers_are_refused():
     I, V = ht.Variable(name='i', trainable=False), ht.Variable(name='v', trainable=False)
     ht.balance_loss_op(ht.Variable(name='x'), I, 8, V)
     assert I.keep_fp32                                # (what a feed under mixed precision goes by)
+
+
+def test_forward_results_that_are_not_whole_are_refused():
+    x, idx, valid, g = _case(10, 9, 2, torch.float32, 'most', 4, 'cpu')
+    r = K.balance_loss(x, idx, 9)
+    K.balance_loss_backward(x, K.BalanceLoss(r.buffer, 9), g)
+    n = r.buffer.numel()
+    for buffer in (r.buffer.to('meta'), r.buffer[:9], r.buffer.int(), torch.zeros(2 * n, dtype=torch.int64)[::2]):
+        with pytest.raises(ValueError):
+            K.balance_loss_backward(x, K.BalanceLoss(buffer, 9), g)

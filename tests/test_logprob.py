@@ -398,3 +398,16 @@ def test_gradient_of_the_longest_row_at_another_alignment():
     assert bool(((d[3000:V - 3000:4099].double() + p).abs() <= step * p).all())
     want = torch.tensor([-math.exp(20.0) * p, -p, 1.0 - p], dtype=torch.float64, device='cuda')
     assert bool(((d[V - 3:].double() - want).abs() <= step * want.abs()).all())
+
+
+def test_forward_results_that_are_not_whole_are_refused():
+    """of another device, strided, or without their ids: the backward pass would read where nothing is"""
+    x, ids, _ = _case(4, 50, torch.float32, 'none', 9, 'cpu')
+    grad, r = torch.zeros(4, 4), K.token_logprob(x, ids, 2)
+    K.token_logprob_backward(x, ids, K.TokenLogProb(r.buffer, r.ids), grad)
+    wide = torch.zeros(4, 12)
+    for buffer, tokens in ((r.buffer.to('meta'), r.ids), (r.buffer, r.ids.to('meta')), (r.buffer, None), (wide[:, ::2], r.ids),
+                           (r.buffer, torch.zeros(4, 4, dtype=torch.int64)[:, ::2]), (r.buffer, r.ids[:2]),
+                           (r.buffer, r.ids.int()), (r.buffer.double(), r.ids)):
+        with pytest.raises(ValueError):
+            K.token_logprob_backward(x, ids, K.TokenLogProb(buffer, tokens), grad)
