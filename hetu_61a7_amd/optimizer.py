@@ -92,6 +92,12 @@ class Optimizer(object):
                           gscale=flat.gscale, seg_off=flat.seg_off, seg_off_host=flat.seg_host,
                           norms_ws=flat.norms_ws, dyn=dyn, **self.hyper(step))
 
+    def check_server_state(self, mode):
+        """the parameter server holds the dense state in 32 bits: refuse another width there"""
+        if self.state_bits != 32:
+            raise ValueError('%s(state_bits=%d): the parameter server holds the dense state (%s)'
+                             % (type(self).__name__, self.state_bits, mode))
+
     def shard_update(self, flat, lo, hi, own, step, dyn=None):
         """ZeRO-1: update parameters [lo, hi) from ``flat.zgrad[own]`` with this rank's state"""
         KO.optimizer_flat(self.mode, flat.param[lo:hi], flat.zgrad[own], flat.s1[own] if flat.s1 is not None else None,
@@ -451,9 +457,7 @@ class OptimizerOp(Op):
         elif self.dp:
             self._make_buckets(dense)
         if self.ps_dense_wanted and self.flat.numel > 0:
-            if opt.state_bits != 32:
-                raise ValueError('%s(state_bits=%d): the parameter server holds the dense state (comm_mode PS)'
-                                 % (type(opt).__name__, opt.state_bits))
+            opt.check_server_state('comm_mode PS')
             from .ps.table import PSDense
             from .ps import PS_KEY_OPT_FLAT
             # key space: node ids are < 2^20; the flat dense key sits above them

@@ -319,6 +319,10 @@ class PipelineSubExecutor(object):
         self.local_grads = {g: i for i, (p, g) in enumerate(local)}
         if not local:
             return
+        # HetPipe: the PS aggregates the replicas' gradients, so no replica all-reduce
+        ps_sync = self.kind == 'hetpipe' and self.config.ps_comm is not None
+        if ps_sync:
+            gop.optimizer.check_server_state('hetpipe')
         opt = copy.copy(gop.optimizer)
         opt.params = [p for p, _ in local]
         op = OptimizerOp.__new__(OptimizerOp)
@@ -328,8 +332,6 @@ class PipelineSubExecutor(object):
         op.bucket_bytes = int(getattr(self.config, 'bucket_mb', 32) * (1 << 20))
         op.ps_dense = None
         op.ps_dense_wanted = False
-        # HetPipe: the PS aggregates the replicas' gradients, so no replica all-reduce
-        ps_sync = self.kind == 'hetpipe' and self.config.ps_comm is not None
         if self.nreplica > 1 and not ps_sync:
             op.comm = self.replica_comms[self.stage]
             op.dp = True
