@@ -50,14 +50,17 @@ def _fused_locations(topk_indices, k, num_experts):
 
 def topkgating(logits, k, capacity_factor, num_tokens, num_experts, embed_dim=None, fused=True, token_mask=None):
     """``token_mask`` [tokens], 0 for padding: the balance loss then counts the other tokens alone
-    (``balance_loss_op``); routing and capacity are the same with and without it."""
+    (``balance_loss_op``); routing, capacity and the shapes are the same with and without it."""
+    native_gate = fused and k <= 8 and num_experts <= 512
     if token_mask is not None:
         _, indices_s, location_s, gates_s, capacity = topkgating(logits, k, capacity_factor, num_tokens, num_experts,
                                                                  embed_dim, fused)
         l_aux, _ = O.balance_loss_op(logits, indices_s, num_experts, token_mask)
+        if not native_gate:          # the op-by-op graph's loss is a scalar without an axis
+            l_aux = O.reduce_sum_op(l_aux, axes=0)
         return l_aux, indices_s, location_s, gates_s, capacity
     capacity = k * math.ceil((num_tokens / num_experts) * capacity_factor)
-    if fused and k <= 8 and num_experts <= 512:
+    if native_gate:
         from ..ops.moe import topk_gating_op
         l_aux, idx, loc, gate_w = topk_gating_op(logits, k, capacity, num_experts)
         return l_aux, [idx], [loc], [gate_w], capacity
