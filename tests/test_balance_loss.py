@@ -301,3 +301,20 @@ def test_moe_layer_with_a_token_mask(k, fused, device):
         assert abs(float(l.reshape(-1)[0]) - loss) <= 200 * U * loss
         # each entry sums 40 products of |x| < 4 with the rows' gradients, each at most k E / 29
         assert np.abs(g - want.numpy()).max() <= 200 * U * 40 * 4 * k * E / 29
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('T,E,k,dt,off', [
+    (30001, 8, 2, torch.float32, 0), (200003, 24, 2, torch.bfloat16, 0), (100003, 60, 4, torch.bfloat16, 0),
+    (100003, 60, 4, torch.float32, 1), (40001, 120, 3, torch.bfloat16, 0), (20001, 161, 6, torch.float32, 0),
+    (9001, 161, 6, torch.bfloat16, 3), (70001, 256, 8, torch.bfloat16, 0), (20001, 256, 8, torch.float32, 2),
+    (10001, 512, 8, torch.bfloat16, 0), (9001, 1000, 4, torch.float32, 0),
+    # gradients and logits larger together than the last-level cache
+    (262500, 256, 8, torch.bfloat16, 0), (140001, 240, 2, torch.float32, 0)])
+def test_many_blocks_of_tokens(T, E, k, dt, off):
+    """the partial sums of up to 512 blocks and every number of lanes a row, masked: values, not only that two
+    calls agree"""
+    wide, idx, valid, g = _case(T, E + (off and 5), k, dt, 'most', T + E, 'cuda')
+    x, idx = wide[:, off:off + E], idx.clamp_max(E - 1)
+    r = K.balance_loss(x, idx, E, valid)
+    _check(x, idx, valid, g, r, K.balance_loss_backward(x, r, g, valid))

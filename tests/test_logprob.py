@@ -411,3 +411,35 @@ def test_forward_results_that_are_not_whole_are_refused():
                            (r.buffer, r.ids.int()), (r.buffer.double(), r.ids)):
         with pytest.raises(ValueError):
             K.token_logprob_backward(x, ids, K.TokenLogProb(buffer, tokens), grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('R,V,pitch,top,dt', [
+    # gradients beyond half the last-level cache, then logits beyond three times it
+    (1101, 61003, 61003, 0, torch.bfloat16), (1101, 61003, 61004, 3, torch.bfloat16), (600, 60001, 60001, 3, torch.float32),
+    (600, 60001, 60003, 0, torch.float32), (6700, 60103, 60103, 2, torch.bfloat16), (6700, 60103, 60112, 0, torch.bfloat16),
+    (3400, 60001, 60001, 0, torch.float32), (3400, 60001, 60002, 2, torch.float32)])
+def test_gradients_larger_than_the_cache(R, V, pitch, top, dt):
+    """rows aligned like the gradient's (pitch = V) and not, of the sizes where the gradient, then the logits too,
+    go past the last-level cache: rows at both ends and between against 64 bits"""
+    g = torch.Generator(device='cuda').manual_seed(R + pitch)
+    x = torch.empty(R, pitch, dtype=dt, device='cuda')
+    for a in range(0, R, 500):
+        x[a:a + 500] = (2 * torch.randn(min(500, R - a), pitch, generator=g, device='cuda')).to(dt)
+    x = x[:, pitch - V:]
+    ids = torch.randint(0, V, (R,), generator=g, device='cuda')
+    ids[2::4] = -1
+    x[5] = -INF
+    grad = torch.randn(R, 2 + top, generator=g, device='cuda')
+    r = K.token_logprob(x, ids, top)
+    d = K.token_logprob_backward(x, ids, r, grad)
+    rows = torch.unique(torch.cat([torch.arange(8), torch.arange(R - 8, R), torch.linspace(8, R - 9, 16).long()])).cuda()
+    part = K.TokenLogProb(r.buffer[rows], r.ids[rows] if top else None)
+    _check(x[rows], ids[rows], top, dt, part, d[rows], grad[rows])
+    # every row: its gradient's sum is 0 but for the roundings of its elements, each at most half a step of
+    # bf16 of itself, and zero for tokens that are not there
+    eps = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -20
+    for a in range(0, R, 500):
+        part = d[a:a + 500].double()
+        assert bool((part.sum(1).abs() <= eps * part.abs().sum(1) + 1e-5 * grad[a:a + 500].double().abs().sum(1)).all())
+        assert not part[ids[a:a + 500] < 0].any()
