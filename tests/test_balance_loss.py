@@ -259,50 +259,6 @@ def test_forward_results_that_are_not_whole_are_refused():
             K.balance_loss_backward(x, K.BalanceLoss(buffer, 9), g)
 
 
-@pytest.mark.parametrize('device', DEVICES)
-@pytest.mark.parametrize('fused', [False, True])
-@pytest.mark.parametrize('k', [1, 2])
-def test_moe_layer_with_a_token_mask(k, fused, device):
-    """MoELayer(x, token_mask): the output of the layer without a mask, the balance loss of the tokens that are
-    not padding with the same shape, and its gradient in the router's weights, against 64 bits"""
-    T, d, E = 40, 8, 4
-    rng = np.random.RandomState(k)
-    xv, wv = rng.randn(T, d).astype(np.float32), rng.randn(d, E).astype(np.float32)
-    on = np.arange(T) < 29
-    ctx = ht.cpu(0) if device == 'cpu' else ht.gpu(0)
-    out = []
-    for mask in (None, on):
-        X, M = ht.Variable(name='x', trainable=False), ht.Variable(name='m', trainable=False)
-        gate = ht.layers.TopKGate(d, T, E, k=k, capacity_factor=float(E), fused=fused, initializer=lambda shape, name: ht.Variable(
-            name=name, value=wv))
-        router = []
-        linear = gate._logits
-        gate._logits = lambda x: router.append(linear(x)) or router[0]
-        experts = [ht.layers.Expert(d, d, bias=False, name='expert%d' % i, initializer=lambda shape, name, i=i: ht.Variable(
-            name=name, value=np.full(shape, 0.01 * (i + 1), np.float32))) for i in range(E)]
-        layer = ht.layers.MoELayer(gate, experts, T, d)
-        y, l_aux = layer(X) if mask is None else layer(X, M)
-        w = [n for n in ht.optim.Optimizer.get_var_list(router[0]) if n.name.startswith('TopK_Gate_linear_weight')]
-        (gw,) = ht.gradients(l_aux, w)
-        ex = ht.Executor({'train': [y, l_aux, gw]}, ctx=ctx)
-        feed = {X: xv} if mask is None else {X: xv, M: mask.astype(np.float32)}
-        out.append([np.asarray(v) for v in ex.run('train', feed_dict=feed, convert_to_numpy_ret_vals=True)])
-    np.testing.assert_array_equal(out[0][0], out[1][0])
-    assert out[0][1].shape == out[1][1].shape
-    W = torch.from_numpy(wv).double().requires_grad_(True)
-    logits = torch.from_numpy(xv).double() @ W
-    top = torch.topk(logits.detach(), k, dim=1)[1]
-    for (_, l, g), valid in zip(out, (np.ones(T, bool), on)):
-        valid = torch.from_numpy(valid)
-        share = torch.bincount(top[valid].reshape(-1), minlength=E).double() / int(valid.sum())
-        loss = E * (share * torch.softmax(logits[valid], 1).mean(0)).sum()
-        (want,) = torch.autograd.grad(loss, W, retain_graph=True)
-        loss = float(loss.detach())
-        assert abs(float(l.reshape(-1)[0]) - loss) <= 200 * U * loss
-        # each entry sums 40 products of |x| < 4 with the rows' gradients, each at most k E / 29
-        assert np.abs(g - want.numpy()).max() <= 200 * U * 40 * 4 * k * E / 29
-
-
 @pytest.mark.gpu
 @pytest.mark.parametrize('T,E,k,dt,off', [
     (30001, 8, 2, torch.float32, 0), (200003, 24, 2, torch.bfloat16, 0), (100003, 60, 4, torch.bfloat16, 0),
