@@ -35,8 +35,9 @@ struct Adam8Args {
 constexpr int kBlock8 = 256;   // elements that share a scale: 8 a lane, half a wave
 constexpr int kLane8 = 8;
 
-// a 32-bit mix (multiply, xor-shift) of a number made from the element's index and the step's
-// seed: the low half rounds m, the high half v
+// a 32-bit mix (multiply, xor-shift; the multipliers and shifts of C. Wellons, "Prospecting for Hash
+// Functions", 2018) of a number made from the element's index and the step's seed: the low half
+// rounds m, the high half v
 __device__ __forceinline__ unsigned round_bits(unsigned h) {
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;

@@ -12,9 +12,13 @@
 // The n largest need no second pass over the row: each thread's largest element is a sample, and
 // the n-th largest sample, T, is a lower bound of the n-th largest element.  Only the n threads
 // whose sample is at least T can hold an element above it; their elements alone are read again,
-// from the cache, and those of at least T (n and a few) are ranked.  Elements compare as one
-// 64-bit key of value and index, so equal values go to the lowest index, whatever their number
-// (the samples as a key of value and granule: a bound on elements all the same).
+// from the cache, and those of at least T (n and a few, where few values tie) are ranked.  Elements
+// compare as one 64-bit key of value and index, so equal values go to the lowest index, whatever
+// their number (the samples as a key of value and granule: a bound on elements all the same).  A row
+// most of whose values tie, or with fewer tokens above -inf than alternatives, has more at the bound:
+// of bf16 rows of 32 KB and more and from 33 alternatives, where four threads share a sample, up to
+// 8 (4 (n - 1) + 1), which the list does not hold.  Such a row is read n times (502 x 131072 bf16, 10
+// tokens above -inf: top 32 70 us, top 64 1.9 ms, and 43 us without a mask).
 //
 // A token outside [0, V) or equal to `ignored` leaves its row unread: zeros, and -1 as top ids.
 // A row of -inf alone has logp -inf, entropy 0 and no gradient.
@@ -626,8 +630,9 @@ static void launch_fwd(const void* logits, int64_t stride, const int64_t* ids, i
   const int64_t bytes = (int64_t)V * sizeof(T);
   // 1024 threads for long rows that are few, or that have alternatives to find (a thread's elements are
   // read again: 1000 x 131072 top 20 57 us, with 256 threads 71 against 63 then); 256 threads else (8192
-  // x 30522: 117 us, with 128 130, with 512 124, all before the gradient went past the cache, 81 since);
-  // a wave for rows that it holds in registers (16384 x 2000 bf16 top 64: 64 us)
+  // x 30522: 117 us, with 128 130, with 512 124, all before the gradient went past the cache, 74 to 81
+  // since); a wave for rows that it holds in registers (16384 x 2000 bf16: 16 us, with 5 alternatives 39,
+  // with 20 44, with 64 64, of which the row's 64-key sort and bit searches are all but the 16)
   if (bytes <= kShortBytes) {
     const dim3 grid = many_blocks((R + kShortWaves - 1) / kShortWaves), block(64 * kShortWaves);
     if (n) hipLaunchKernelGGL((token_logprob_short_k<T, true>), grid, block, 0, st, (const T*)logits, stride, ids, R, V, n, ignored, out, top);
